@@ -88,6 +88,28 @@ _SIGNATURES = {
     "hx_matmul_splits": (_c.c_int, [_c.c_int64] * 7 + [_c.c_int, _c.c_int]),
     "hx_attention": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int64] * 5 + [_c.c_int, _c.c_void_p]),
     "hx_attention_path": (_c.c_int, [_c.c_int64] * 4 + [_c.c_int] + [_c.c_void_p] * 4),
+    "hx_rms_norm_int8": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_float, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64,
+         _c.c_int64, _c.c_int, _c.c_void_p],
+    ),
+    "hx_int8_quantize_per_token": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_int, _c.c_void_p],
+    ),
+    "hx_int8_gemm": (
+        _c.c_int,
+        [_c.c_void_p] * 3 + [_c.c_int64] * 7 + [_c.c_void_p] * 3 + [_c.c_int, _c.c_int, _c.c_void_p, _c.c_size_t, _c.c_void_p],
+    ),
+    "hx_int8_gemm_workspace_bytes": (_c.c_size_t, [_c.c_int64] * 6 + [_c.c_void_p] * 2),
+    "hx_kv4_write": (_c.c_int, [_c.c_void_p] * 7 + [_c.c_int] + [_c.c_int64] * 9 + [_c.c_int, _c.c_void_p]),
+    "hx_kv4_read": (_c.c_int, [_c.c_void_p] * 5 + [_c.c_int] + [_c.c_void_p] * 2 + [_c.c_int64] * 5 + [_c.c_int, _c.c_void_p]),
+    "hx_kv4_attention": (
+        _c.c_int,
+        [_c.c_void_p] + [_c.c_int64] * 2 + [_c.c_void_p] * 5 + [_c.c_int64] + [_c.c_void_p] * 3 + [_c.c_int64] * 9
+        + [_c.c_float, _c.c_int, _c.c_int, _c.c_void_p, _c.c_size_t, _c.c_void_p],
+    ),
+    "hx_kv4_attention_workspace_bytes": (_c.c_size_t, [_c.c_int64] * 8 + [_c.c_int]),
     "hx_clock_probe": (_c.c_int, [_c.c_void_p, _c.c_int64, _c.c_void_p]),
     "hx_matmul_path": (_c.c_int, [_c.c_int64] * 7 + [_c.c_int, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p]),
 }

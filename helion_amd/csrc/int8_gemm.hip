@@ -1,0 +1,412 @@
+// Product of 8-bit integers for gfx950 with a scale for each row of A (token) and each column of B (channel):
+//   C[M,N] = cast( (sum_k A[m,k] B[k,n]) * scale_a[m] * scale_b[n] + bias[n] )
+// The sum is exact (32-bit integers, K <= 131071: 128 * 128 * K stays below 2^31); scales and bias are applied in fp32.
+//
+// The kernels read K-contiguous rows of A and of B^T in pieces of 16 bytes.  Operands that are not like that (another
+// stride order, K % 16 != 0, unaligned rows) are copied once into the workspace with rows padded to a multiple of 128; a K
+// that is a multiple of 16 but not of 128 needs the copy of A only: its padding is zeros, and what stands in the other
+// factor of a zero does not matter for integers, so B's rows are simply read on (clamped to the end of the matrix).
+#include "hx_common.h"
+
+#include <type_traits>
+
+#define I8_BK 128  // bytes of k per tile row
+
+struct I8Args {
+  const uint8_t *a, *b;  // rows of A and of B^T, K contiguous
+  void* c;
+  const float *sa, *sb;
+  const void* bias;
+  int M, N, nk;  // nk: k-tiles of 128
+  long lda, ldb, ldc;
+  int bias_dt;
+  int tiles_m, bn, kt_per_split;
+  uint32_t b_max;  // last byte offset of B^T a 16-byte read may start at
+};
+
+__device__ __forceinline__ v4i i8_mfma(v4i a, v4i b, v4i c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ float i8_bias(const void* bias, int dt, long n) {
+  return dt == HX_F32 ? ((const float*)bias)[n] : dt == HX_BF16 ? (float)((const __bf16*)bias)[n] : (float)((const _Float16*)bias)[n];
+}
+
+// ------------------------------------------------------------------------------------------
+// tile: BM x 128 outputs per workgroup, 4 waves (2 x 2) of BM/2 x 64.  Ring of NS k-tiles in the LDS, filled by DMA
+// (eight rows x 128 bytes per instruction, 16-byte chunk c of row r at position c ^ ((r >> 1) & 7)); a 16x16x64 MFMA takes
+// 16 bytes per lane, so a k-tile is two of them per pair of blocks: lane group g multiplies chunks 2kq and 2kq+1 with
+// kq = 0, 3, 1, 2 (the order in which the 16-byte reads of a wave meet no bank twice).
+// split-K (kt_per_split): workgroup row blockIdx.y adds up its k-tiles into its own slab of 32-bit integers.
+// KT: K is not a multiple of 128 (A padded, B read on).
+// ------------------------------------------------------------------------------------------
+template <int OUT, int BM, bool KT, bool SPLIT>
+__global__ __launch_bounds__(256) void hx_int8_gemm_tile(I8Args p) {
+  constexpr int NS = BM == 64 ? 6 : 4;
+  constexpr int STAGE = (BM + 128) * 128;
+  constexpr int WMB = BM / 32;
+  constexpr int AJ = BM / 32, IPW = AJ + 4;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[NS][STAGE];
+
+  const int kt0 = SPLIT ? p.kt_per_split * (int)blockIdx.y : 0;
+  const int nk = SPLIT ? min(p.kt_per_split, p.nk - kt0) : p.nk;
+  // 256 consecutive tiles of a raster of eight tile rows at a time, in blocks of 32 per XCD (workgroup i runs on XCD i % 8)
+  int tm, tn;
+  {
+    const int nwg = gridDim.x, wg = blockIdx.x, chunk = wg >> 8, tiles_n = nwg / p.tiles_m;
+    const int rem = nwg & 255, l = wg & 255;
+    const int tile = chunk < (nwg >> 8) ? (chunk << 8) + ((wg & 7) << 5) + ((wg >> 3) & 31)
+                     : (rem & 7) == 0   ? (chunk << 8) + (l & 7) * (rem >> 3) + (l >> 3)
+                                        : wg;
+    const int group = 8 * tiles_n, first = (tile / group) * 8, gm = min(p.tiles_m - first, 8);
+    tm = first + (tile % group) % gm;
+    tn = (tile % group) / gm;
+  }
+  const long m0 = (long)tm * BM, n0 = (long)tn * p.bn;
+  const int nlast = (int)min(n0 + p.bn, (long)p.N) - 1;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = w >> 1, wn = w & 1;
+
+  // ---- DMA: instruction j of an operand covers rows 8j .. 8j+7; wave w issues j = w, w+4, ...
+  const int lrow = lane >> 3, lpos = lane & 7;
+  const uint32_t chunk = (uint32_t)((lpos ^ ((4 * (w & 1) + (lrow >> 1)) & 7)) * 16);
+  uint32_t a_vo[AJ], b_vo[4];
+#pragma unroll
+  for (int jj = 0; jj < AJ; ++jj) a_vo[jj] = (uint32_t)min((int)m0 + 8 * (w + 4 * jj) + lrow, p.M - 1) * (uint32_t)p.lda + chunk;
+#pragma unroll
+  for (int jj = 0; jj < 4; ++jj) b_vo[jj] = (uint32_t)min((int)n0 + 8 * (w + 4 * jj) + lrow, nlast) * (uint32_t)p.ldb + chunk;
+  const uint32_t lds0 = hx_lds_addr(&smem[0][0]);
+  // past the last k-tile: that one again, so that every step issues IPW instructions and the counted waits stay exact
+  auto issue_one = [&](int kt, int i) {
+    const long t = (long)(kt0 + min(kt, nk - 1)) * I8_BK;
+    const uint32_t base = lds0 + (uint32_t)(kt % NS) * STAGE;
+    if (i < AJ) hx_g2l16_s(hx_uniform_ptr(p.a + t), a_vo[i], base + (w + 4 * i) * 1024);
+    else if (KT) hx_g2l16_s(hx_uniform_ptr(p.b), min(b_vo[i - AJ] + (uint32_t)t, p.b_max), base + BM * 128 + (w + 4 * (i - AJ)) * 1024);
+    else hx_g2l16_s(hx_uniform_ptr(p.b + t), b_vo[i - AJ], base + BM * 128 + (w + 4 * (i - AJ)) * 1024);
+  };
+
+  const int r16 = lane & 15, gq = lane >> 4;
+  const int kq = (gq >> 1) ^ ((gq & 1) * 3);
+  const int x16 = ((2 * kq) ^ ((r16 >> 1) & 7)) * 16;
+  const int a_base = (wm * (BM / 2) + r16) * 128, b_base = BM * 128 + (wn * 64 + r16) * 128;
+  v4i fa[WMB][2], fb[4][2];
+  auto load_a = [&](int f, int kt) {
+    const uint8_t* st = &smem[kt % NS][0] + a_base + f * 2048;
+    fa[f][0] = *(const v4i*)(st + x16), fa[f][1] = *(const v4i*)(st + (x16 ^ 16));
+  };
+  auto load_b = [&](int f, int kt) {
+    const uint8_t* st = &smem[kt % NS][0] + b_base + f * 2048;
+    fb[f][0] = *(const v4i*)(st + x16), fb[f][1] = *(const v4i*)(st + (x16 ^ 16));
+  };
+  // acc[bj][bi][r] is C[m0 + wm*BM/2 + 16 bi + lane%16][n0 + wn*64 + 16 bj + 4*(lane/16) + r]
+  v4i acc[4][WMB];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < WMB; ++j) acc[i][j] = (v4i){0, 0, 0, 0};
+
+  // One k-tile: its MFMAs row block by row block; a fragment takes the next tile's rows as soon as its last MFMA is out,
+  // one DMA instruction follows every MFMA pair.
+  auto step = [&](int kt) {
+    __builtin_amdgcn_s_waitcnt(hx_vmcnt_imm((NS - 2) * IPW));  // this wave's part of tile kt+1 has landed
+    __syncthreads();  // ... everybody's has, and every wave has read tile kt out of its stage
+#pragma unroll
+    for (int i = 0; i < 4 * WMB; ++i) {
+      const int bj = i & 3, bi = i >> 2;
+      acc[bj][bi] = i8_mfma(fb[bj][0], fa[bi][0], acc[bj][bi]);
+      acc[bj][bi] = i8_mfma(fb[bj][1], fa[bi][1], acc[bj][bi]);
+      if (i < IPW) issue_one(kt + NS, i);
+      if (bj == 3) load_a(bi, kt + 1);
+      if (bi == WMB - 1) load_b(bj, kt + 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  static_assert(4 * WMB >= IPW, "every DMA instruction of a k-tile has an MFMA to follow");
+  for (int t = 0; t < NS; ++t)
+#pragma unroll
+    for (int i = 0; i < IPW; ++i) issue_one(t, i);
+  __builtin_amdgcn_s_waitcnt(hx_vmcnt_imm((NS - 1) * IPW));
+  __syncthreads();
+#pragma unroll
+  for (int f = 0; f < WMB; ++f) load_a(f, 0);
+#pragma unroll
+  for (int f = 0; f < 4; ++f) load_b(f, 0);
+  for (int kt = 0; kt < nk; ++kt) step(kt);
+  HX_WAIT_VM0();  // no DMA may still be writing this workgroup's LDS when it ends
+
+  if (SPLIT) {
+    int* C = (int*)p.c + (long)blockIdx.y * p.M * p.N;
+#pragma unroll
+    for (int bi = 0; bi < WMB; ++bi) {
+      const long m = m0 + wm * (BM / 2) + 16 * bi + r16;
+      if (m >= p.M) continue;
+#pragma unroll
+      for (int bj = 0; bj < 4; ++bj) {
+        const long n = n0 + wn * 64 + 16 * bj + 4 * gq;
+        int* dst = C + m * p.N + n;
+        if (n + 3 <= nlast && (p.N & 3) == 0) {
+          *(v4i*)dst = acc[bj][bi];
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (n + r <= nlast) dst[r] = acc[bj][bi][r];
+        }
+      }
+    }
+    return;
+  }
+  typedef typename OutT<OUT>::T out_t;
+  typedef out_t ov4 __attribute__((ext_vector_type(4)));
+  out_t* C = (out_t*)p.c;
+  const bool vec_ok = p.ldc % 4 == 0 && ((uintptr_t)C & (4 * sizeof(out_t) - 1)) == 0;
+  v4f sb[4], add[4];
+#pragma unroll
+  for (int bj = 0; bj < 4; ++bj)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const long n = min(n0 + wn * 64 + 16 * bj + 4 * gq + r, (long)nlast);
+      sb[bj][r] = p.sb[n];
+      add[bj][r] = p.bias ? i8_bias(p.bias, p.bias_dt, n) : 0.f;
+    }
+#pragma unroll
+  for (int bi = 0; bi < WMB; ++bi) {
+    const long m = m0 + wm * (BM / 2) + 16 * bi + r16;
+    if (m >= p.M) continue;
+    const float sa = p.sa[m];
+#pragma unroll
+    for (int bj = 0; bj < 4; ++bj) {
+      const long n = n0 + wn * 64 + 16 * bj + 4 * gq;
+      out_t* dst = C + m * p.ldc + n;
+      ov4 o;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = (out_t)((float)acc[bj][bi][r] * sa * sb[bj][r] + add[bj][r]);
+      if (n + 3 <= nlast && vec_ok) {
+        *(ov4*)dst = o;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (n + r <= nlast) dst[r] = o[r];
+      }
+    }
+  }
+}
+
+// split-K: C = cast(sum over the slabs [split][M][N] * scales + bias); one thread per four columns
+template <int OUT>
+__global__ __launch_bounds__(256) void hx_int8_gemm_split_reduce(I8Args p, const int* __restrict__ part, int splits) {
+  typedef typename OutT<OUT>::T out_t;
+  const int n4 = (p.N + 3) >> 2;
+  const long id = (long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= (long)p.M * n4) return;
+  const long m = id / n4, n = (id % n4) * 4;
+  int acc[4] = {0, 0, 0, 0};
+  for (int s = 0; s < splits; ++s)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < p.N) acc[r] += part[((long)s * p.M + m) * p.N + n + r];
+  const float sa = p.sa[m];
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (n + r < p.N)
+      ((out_t*)p.c)[m * p.ldc + n + r] = (out_t)((float)acc[r] * sa * p.sb[n + r] + (p.bias ? i8_bias(p.bias, p.bias_dt, n + r) : 0.f));
+}
+
+// src[r * sr + k * sk] -> dst[r][ld], zeros behind K.  Rows of contiguous bytes: 16 at a time whatever their alignment.
+__global__ __launch_bounds__(256) void hx_int8_pack_rows(const uint8_t* __restrict__ src, uint8_t* __restrict__ dst, long rows, int K, long sr,
+                                                        int ld) {
+  const int per = ld >> 4;
+  const long id = (long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= rows * per) return;
+  const long r = id / per;
+  const int k = (int)(id % per) * 16;
+  const uint8_t* s = src + r * sr + k;
+  typedef int v4iu __attribute__((ext_vector_type(4), aligned(1)));
+  v4i v = {0, 0, 0, 0};
+  if (k + 16 <= K) {
+    v = *(const v4iu*)s;
+  } else {
+    for (int e = 0; e < 16; ++e)
+      if (k + e < K) ((uint8_t*)&v)[e] = s[e];
+  }
+  *(v4i*)(dst + r * ld + k) = v;
+}
+// any strides, through a 64 x 64 tile
+__global__ __launch_bounds__(256) void hx_int8_pack_any(const uint8_t* __restrict__ src, uint8_t* __restrict__ dst, int rows, int K, long sr,
+                                                       long sk, int ld) {
+  __shared__ uint8_t t[64][64 + 4];
+  const int r0 = blockIdx.x * 64, k0 = blockIdx.y * 64, x = threadIdx.x & 63;
+  for (int y = threadIdx.x >> 6; y < 64; y += 4) {
+    const int r = r0 + x, k = k0 + y;
+    t[y][x] = r < rows && k < K ? src[r * sr + k * sk] : (uint8_t)0;
+  }
+  __syncthreads();
+  for (int y = threadIdx.x >> 6; y < 64; y += 4) {
+    const int r = r0 + y, k = k0 + x;
+    if (r < rows && k < ld) dst[(long)r * ld + k] = t[x][y];
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------
+struct I8Plan {
+  bool copy_a, copy_b, tail;  // tail: K % 128 != 0 with B read in place
+  int64_t ka;                 // padded row length of the copies
+  int bm, bn, splits, kt_per_split;
+  size_t a_off, b_off, part_off, bytes;
+};
+
+static I8Plan i8_plan(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb_k, int64_t ldb_n, bool a_aligned, bool b_aligned) {
+  I8Plan p;
+  p.ka = (K + I8_BK - 1) / I8_BK * I8_BK;
+  const bool b_rows = ldb_k == 1 && ldb_n >= K && ldb_n % 16 == 0 && b_aligned && N * ldb_n <= (1LL << 32) - 512;
+  p.copy_b = !(b_rows && K % 16 == 0);
+  p.tail = !p.copy_b && K % I8_BK != 0;
+  p.copy_a = !(K % I8_BK == 0 && lda % 16 == 0 && a_aligned && M * lda < (1LL << 32));
+  p.bm = M <= 64 ? 64 : 128;
+  p.bn = 128;
+  const int64_t tiles = ((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn), nk = p.ka / I8_BK;
+  // Few tiles and a long K: the k-tiles of a tile are divided among workgroups, eight at least for each, and the partial
+  // sums stay below 32 MB.
+  int64_t s = hx_cu_count() / tiles;
+  if (s > nk / 8) s = nk / 8;
+  while (s > 1 && s * M * N * 4 > (32LL << 20)) --s;
+  p.splits = 1, p.kt_per_split = 0;
+  if (s > 1) {
+    p.kt_per_split = (int)((nk + s - 1) / s);
+    p.splits = (int)((nk + p.kt_per_split - 1) / p.kt_per_split);
+  }
+  size_t at = 0;
+  auto take = [&](bool want, int64_t bytes) {
+    const size_t here = at;
+    if (want) at += ((size_t)bytes + 255) & ~(size_t)255;
+    return here;
+  };
+  p.a_off = take(p.copy_a, M * p.ka);
+  p.b_off = take(p.copy_b, N * p.ka);
+  p.part_off = take(p.splits > 1, (int64_t)p.splits * M * N * 4);
+  p.bytes = at;
+  return p;
+}
+
+static int i8_check(const char* who, int64_t M, int64_t N, int64_t K) {
+  if (M < 0 || N < 0 || K < 0) {
+    hx_set_error("%s: negative size M=%lld N=%lld K=%lld", who, (long long)M, (long long)N, (long long)K);
+    return HX_ERR_BAD_ARG;
+  }
+  if (K > 131071) {
+    hx_set_error("%s: K=%lld: a sum of more than 131071 products does not fit in 32 bits", who, (long long)K);
+    return HX_ERR_UNSUPPORTED;
+  }
+  const int64_t ka = (K + I8_BK - 1) / I8_BK * I8_BK;
+  if (M >= (1LL << 31) - 256 || N >= (1LL << 31) - 256 || (M + 63) / 64 * ((N + 127) / 128) >= (1LL << 31) || M * ka >= (1LL << 32) ||
+      N * ka >= (1LL << 32)) {
+    hx_set_error("%s: operands of 4 GB or more", who);
+    return HX_ERR_UNSUPPORTED;
+  }
+  return 0;
+}
+
+extern "C" size_t hx_int8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb_k, int64_t ldb_n, const void* a,
+                                               const void* b) {
+  if (M <= 0 || N <= 0 || K <= 0 || i8_check("hx_int8_gemm", M, N, K) != 0) return 0;
+  return i8_plan(M, N, K, lda, ldb_k, ldb_n, ((uintptr_t)a & 15) == 0, ((uintptr_t)b & 15) == 0).bytes;
+}
+
+static void i8_pack(const void* src, uint8_t* dst, int64_t rows, int64_t K, int64_t sr, int64_t sk, int64_t ld, hipStream_t s) {
+  if (sk == 1)
+    hx_launch(hx_int8_pack_rows, dim3((unsigned)((rows * (ld / 16) + 255) / 256)), dim3(256), 0, s, (const uint8_t*)src, dst, (long)rows, (int)K,
+              (long)sr, (int)ld);
+  else
+    hx_launch(hx_int8_pack_any, dim3((unsigned)((rows + 63) / 64), (unsigned)((ld + 63) / 64)), dim3(256), 0, s, (const uint8_t*)src, dst,
+              (int)rows, (int)K, (long)sr, (long)sk, (int)ld);
+}
+
+template <int OUT, int BM>
+static void i8_launch_tile(const I8Args& a, const I8Plan& p, dim3 grid, hipStream_t s) {
+  if (p.splits > 1) {
+    if (p.tail) hx_launch(hx_int8_gemm_tile<HX_F32, BM, true, true>, grid, dim3(256), 0, s, a);
+    else hx_launch(hx_int8_gemm_tile<HX_F32, BM, false, true>, grid, dim3(256), 0, s, a);
+  } else {
+    if (p.tail) hx_launch(hx_int8_gemm_tile<OUT, BM, true, false>, grid, dim3(256), 0, s, a);
+    else hx_launch(hx_int8_gemm_tile<OUT, BM, false, false>, grid, dim3(256), 0, s, a);
+  }
+}
+
+template <int OUT>
+static void i8_launch(I8Args a, const I8Plan& p, void* ws, hipStream_t s) {
+  a.tiles_m = (a.M + p.bm - 1) / p.bm, a.bn = p.bn, a.kt_per_split = p.kt_per_split;
+  const dim3 grid((unsigned)(a.tiles_m * ((a.N + p.bn - 1) / p.bn)), (unsigned)p.splits);
+  void* c = a.c;
+  if (p.splits > 1) a.c = (uint8_t*)ws + p.part_off;
+  if (p.bm == 64) i8_launch_tile<OUT, 64>(a, p, grid, s);
+  else i8_launch_tile<OUT, 128>(a, p, grid, s);
+  if (p.splits > 1) {
+    const int* part = (const int*)a.c;
+    a.c = c;
+    const long quads = (long)a.M * ((a.N + 3) / 4);
+    hx_launch(hx_int8_gemm_split_reduce<OUT>, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, a, part, p.splits);
+  }
+}
+
+extern "C" int hx_int8_gemm(const void* a, const void* b, void* c, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb_k, int64_t ldb_n,
+                            int64_t ldc, const float* scale_a, const float* scale_b, const void* bias, int bias_dtype, int out_dtype,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "hx_int8_gemm";
+  int rc = i8_check(who, M, N, K);
+  if (rc != 0) return rc;
+  if (out_dtype != HX_F16 && out_dtype != HX_BF16 && out_dtype != HX_F32) {
+    hx_set_error("%s: out_dtype must be HX_F16, HX_BF16 or HX_F32, got %d", who, out_dtype);
+    return HX_ERR_BAD_ARG;
+  }
+  if (bias && bias_dtype != HX_F16 && bias_dtype != HX_BF16 && bias_dtype != HX_F32) {
+    hx_set_error("%s: bias dtype must be HX_F16, HX_BF16 or HX_F32, got %d", who, bias_dtype);
+    return HX_ERR_BAD_ARG;
+  }
+  if (M == 0 || N == 0) return 0;
+  if (K == 0) {
+    hx_set_error("%s: K = 0", who);
+    return HX_ERR_UNSUPPORTED;
+  }
+  if (!a || !b || !c || !scale_a || !scale_b) {
+    hx_set_error("%s: null pointer", who);
+    return HX_ERR_BAD_ARG;
+  }
+  if (lda < K || ldc < N || ldb_k < 1 || ldb_n < 1) {
+    hx_set_error("%s: leading dimension smaller than row length (lda=%lld K=%lld ldc=%lld N=%lld ldb=%lld,%lld)", who, (long long)lda,
+                 (long long)K, (long long)ldc, (long long)N, (long long)ldb_k, (long long)ldb_n);
+    return HX_ERR_BAD_ARG;
+  }
+  const uintptr_t oes = out_dtype == HX_F32 ? 4 : 2, bes = bias_dtype == HX_F32 ? 4 : 2;
+  if (((uintptr_t)c & (oes - 1)) || (bias && ((uintptr_t)bias & (bes - 1))) || (((uintptr_t)scale_a | (uintptr_t)scale_b) & 3)) {
+    hx_set_error("%s: pointers must be aligned to their elements", who);
+    return HX_ERR_UNSUPPORTED;
+  }
+  const I8Plan p = i8_plan(M, N, K, lda, ldb_k, ldb_n, ((uintptr_t)a & 15) == 0, ((uintptr_t)b & 15) == 0);
+  if (p.bytes && (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255))) {
+    hx_set_error("%s: workspace must be 256-byte aligned and at least %zu bytes (got %zu)", who, p.bytes, workspace_bytes);
+    return HX_ERR_WORKSPACE;
+  }
+  hipStream_t s = (hipStream_t)stream;
+  uint8_t* ws = (uint8_t*)workspace;
+  I8Args g;
+  g.a = (const uint8_t*)a, g.b = (const uint8_t*)b, g.c = c, g.sa = scale_a, g.sb = scale_b, g.bias = bias, g.bias_dt = bias_dtype;
+  g.M = (int)M, g.N = (int)N, g.nk = (int)(p.ka / I8_BK), g.lda = lda, g.ldb = ldb_n, g.ldc = ldc;
+  if (p.copy_a) {
+    i8_pack(a, ws + p.a_off, M, K, lda, 1, p.ka, s);
+    g.a = ws + p.a_off, g.lda = p.ka;
+  }
+  if (p.copy_b) {
+    i8_pack(b, ws + p.b_off, N, K, ldb_n, ldb_k, p.ka, s);
+    g.b = ws + p.b_off, g.ldb = p.ka;
+  }
+  g.b_max = (uint32_t)((N - 1) * g.ldb + (p.copy_b ? p.ka : K) - 16);
+  if (out_dtype == HX_F16) i8_launch<HX_F16>(g, p, ws, s);
+  else if (out_dtype == HX_BF16) i8_launch<HX_BF16>(g, p, ws, s);
+  else i8_launch<HX_F32>(g, p, ws, s);
+  const hipError_t e = hx_launch_status();
+  if (e != hipSuccess) {
+    hx_set_error("%s: launch failed: %s", who, hipGetErrorString(e));
+    return (int)e;
+  }
+  return 0;
+}

@@ -36,6 +36,31 @@ def _require_cuda(*tensors: torch.Tensor) -> None:
             raise RuntimeError("helion_amd ops run on the GPU only (HIP kernels); got a tensor on " + str(t.device))
 
 
+def _one_device(who: str, first: torch.Tensor, *rest: torch.Tensor | None) -> None:
+    for t in rest:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{who}: tensors on {first.device} and {t.device}")
+
+
+class _on:
+    """The device whose tensors a call works on is the current one inside the block (a launch goes to the current device,
+    the stream handle alone does not move it).  Costs one query where it already is."""
+
+    __slots__ = ("index", "old")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.old = torch.cuda.current_device()
+        if self.old != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.old != self.index:
+            torch.cuda.set_device(self.old)
+
+
 # ------------------------------------------------------------------------------ fp8 gemm
 def _fp8_gemm_impl(x: torch.Tensor, y: torch.Tensor, scale_a: torch.Tensor | None, scale_b: torch.Tensor | None,
                 out_dtype: torch.dtype) -> torch.Tensor:
@@ -395,6 +420,309 @@ def _(q, k, v):
     return torch.empty_like(q, memory_format=torch.contiguous_format)
 
 
+# ------------------------------------------------------------------------------ rows to 8-bit integers, with and without a norm
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x as [rows, width] with the elements of a row contiguous, without a copy where its strides allow that."""
+    x = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        x = x.contiguous()
+    return x
+
+
+def _check_rows(who: str, x: torch.Tensor) -> None:
+    if x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TypeError(f"{who} expects float16/bfloat16/float32, got {x.dtype}")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 65536:
+        raise ValueError(f"{who} expects rows of 1 to 65536 elements, got shape {tuple(x.shape)}")
+
+
+def _rms_norm_int8_impl(x: torch.Tensor, weight: torch.Tensor, eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+    return _rms_norm_int8_any(x, None, weight, eps)[:2]
+
+
+def _add_rms_norm_int8_impl(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
+                            eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _rms_norm_int8_any(x, residual, weight, eps)
+
+
+def _rms_norm_int8_any(x, residual, weight, eps):
+    _require_cuda(x, residual, weight)
+    _check_rows("rms_norm_int8", x)
+    width = x.shape[-1]
+    if weight.shape != (width,) or weight.dtype != x.dtype:
+        raise ValueError(f"rms_norm_int8: weight must be [{width}] of {x.dtype}, got {tuple(weight.shape)} of {weight.dtype}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError(f"rms_norm_int8: residual must be {tuple(x.shape)} of {x.dtype}, got {tuple(residual.shape)} of {residual.dtype}")
+    _one_device("rms_norm_int8", x, residual, weight)
+    x2, dev = _rows(x), x.device
+    r2 = _rows(residual) if residual is not None else None
+    weight = weight.contiguous()
+    rows = x2.shape[0]
+    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
+    scale = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=dev)
+    h = torch.empty(x.shape, dtype=x.dtype, device=dev) if residual is not None else None
+    if rows:
+        with _on(dev):
+            rc = _lib.load().hx_rms_norm_int8(x2.data_ptr(), x2.stride(0), r2.data_ptr() if r2 is not None else None,
+                                              r2.stride(0) if r2 is not None else 0, weight.data_ptr(), eps,
+                                              h.data_ptr() if h is not None else None, q.data_ptr(), scale.data_ptr(), rows, width,
+                                              _DT[x.dtype], _stream_ptr(dev))
+        _lib.check(rc, "hx_rms_norm_int8")
+    return q, scale, h
+
+
+rms_norm_int8_op = torch.library.custom_op("helion_amd::rms_norm_int8", mutates_args=())(_rms_norm_int8_impl)
+add_rms_norm_int8_op = torch.library.custom_op("helion_amd::add_rms_norm_int8", mutates_args=())(_add_rms_norm_int8_impl)
+
+
+@rms_norm_int8_op.register_fake
+def _(x, weight, eps):
+    return x.new_empty(x.shape, dtype=torch.int8), x.new_empty((*x.shape[:-1], 1), dtype=torch.float32)
+
+
+@add_rms_norm_int8_op.register_fake
+def _(x, residual, weight, eps):
+    return (x.new_empty(x.shape, dtype=torch.int8), x.new_empty((*x.shape[:-1], 1), dtype=torch.float32),
+            x.new_empty(x.shape))
+
+
+def _int8_quantize_impl(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    _require_cuda(x)
+    _check_rows("int8_quantize_per_token", x)
+    x2, dev = _rows(x), x.device
+    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
+    scale = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=dev)
+    if x2.shape[0]:
+        with _on(dev):
+            rc = _lib.load().hx_int8_quantize_per_token(x2.data_ptr(), x2.stride(0), q.data_ptr(), scale.data_ptr(), x2.shape[0],
+                                                        x2.shape[1], _DT[x.dtype], _stream_ptr(dev))
+        _lib.check(rc, "hx_int8_quantize_per_token")
+    return q, scale
+
+
+int8_quantize_op = torch.library.custom_op("helion_amd::int8_quantize_per_token", mutates_args=())(_int8_quantize_impl)
+
+
+@int8_quantize_op.register_fake
+def _(x):
+    return x.new_empty(x.shape, dtype=torch.int8), x.new_empty((*x.shape[:-1], 1), dtype=torch.float32)
+
+
+# ------------------------------------------------------------------------------ int8 gemm
+def _int8_gemm_impl(x: torch.Tensor, y: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor, bias: torch.Tensor | None,
+                    out_dtype: torch.dtype) -> torch.Tensor:
+    _require_cuda(x, y, scale_a, scale_b, bias)
+    if x.dtype != torch.int8 or y.dtype != torch.int8:
+        raise TypeError(f"int8_gemm expects int8 operands, got {x.dtype} and {y.dtype}")
+    if x.dim() != 2 or y.dim() != 2:
+        raise ValueError("int8_gemm expects 2-D operands")
+    m, k = x.shape
+    k2, n = y.shape
+    if k != k2:
+        raise ValueError(f"int8_gemm: size mismatch {k} != {k2}")
+    if out_dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TypeError(f"unsupported out_dtype {out_dtype}")
+    if scale_a.dtype != torch.float32 or scale_b.dtype != torch.float32:
+        raise TypeError("int8_gemm: scales must be float32")
+    if scale_a.numel() != m or scale_b.numel() != n:
+        raise ValueError(f"int8_gemm: scale_a must have {m} elements and scale_b {n}, got {scale_a.numel()} and {scale_b.numel()}")
+    if bias is not None and (bias.numel() != n or bias.dtype not in (torch.float16, torch.bfloat16, torch.float32)):
+        raise ValueError(f"int8_gemm: bias must be {n} float16/bfloat16/float32 elements, got {tuple(bias.shape)} of {bias.dtype}")
+    _one_device("int8_gemm", x, y, scale_a, scale_b, bias)
+    dev = x.device
+    out = torch.empty((m, n), dtype=out_dtype, device=dev)
+    if m == 0 or n == 0:
+        return out
+    if k == 0:
+        raise ValueError("int8_gemm: K = 0")
+    x = _rows(x)
+    lda = x.stride(0) if m > 1 else k
+    ldb_k = y.stride(0) if k > 1 else 1
+    ldb_n = y.stride(1) if n > 1 else max(k, 1)
+    if ldb_k < 1 or ldb_n < 1:  # an expanded operand
+        y = y.t().contiguous().t()
+        ldb_k, ldb_n = 1, k
+    scale_a, scale_b = scale_a.contiguous(), scale_b.contiguous()
+    bias = bias.contiguous() if bias is not None else None
+    lib = _lib.load()
+    xp, yp = x.data_ptr(), y.data_ptr()
+    with _on(dev):
+        ws_bytes = lib.hx_int8_gemm_workspace_bytes(m, n, k, lda, ldb_k, ldb_n, xp, yp)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        rc = lib.hx_int8_gemm(xp, yp, out.data_ptr(), m, n, k, lda, ldb_k, ldb_n, n, scale_a.data_ptr(), scale_b.data_ptr(),
+                              bias.data_ptr() if bias is not None else None, _DT[bias.dtype] if bias is not None else 0, _DT[out_dtype],
+                              ws.data_ptr() if ws is not None else None, ws_bytes, _stream_ptr(dev))
+    _lib.check(rc, "hx_int8_gemm")
+    return out
+
+
+int8_gemm_op = torch.library.custom_op("helion_amd::int8_gemm", mutates_args=())(_int8_gemm_impl)
+
+
+@int8_gemm_op.register_fake
+def _(x, y, scale_a, scale_b, bias, out_dtype):
+    return x.new_empty((x.shape[0], y.shape[1]), dtype=out_dtype)
+
+
+# ------------------------------------------------------------------------------ key/value cache in 4 bits
+def _check_cache(who: str, kc: torch.Tensor, ks: torch.Tensor, vc: torch.Tensor, vs: torch.Tensor) -> tuple[int, int, int, int]:
+    """(pages, heads, page, head_dim) of a cache whose four tensors fit together."""
+    if any(t.dtype != torch.uint8 for t in (kc, ks, vc, vs)):
+        raise TypeError(f"{who}: the cache's tensors must be uint8")
+    if kc.dim() != 4:
+        raise ValueError(f"{who}: k must be [pages, heads, page, head_dim / 2], got {tuple(kc.shape)}")
+    pages, heads, page, half = kc.shape
+    d = 2 * half
+    if d not in (64, 128, 256):
+        raise ValueError(f"{who}: head_dim must be 64, 128 or 256, got {d}")
+    if page < 16 or page > 1024 or page & (page - 1):
+        raise ValueError(f"{who}: pages hold a power of two from 16 to 1024 tokens, got {page}")
+    if (ks.shape != (pages, heads, page, d // 32) or vc.shape != (pages, heads, page // 4, 16, 4, d // 32)
+            or vs.shape != (pages, heads, page // 4, d // 32, 4)):
+        raise ValueError(f"{who}: the cache's tensors do not fit together: {tuple(kc.shape)} {tuple(ks.shape)} {tuple(vc.shape)} {tuple(vs.shape)}")
+    if not (kc.is_contiguous() and ks.is_contiguous() and vc.is_contiguous() and vs.is_contiguous()):
+        raise ValueError(f"{who}: the cache's tensors must be contiguous")
+    return pages, heads, page, d
+
+
+def _check_slots(who: str, slots: torch.Tensor, tokens: int | None = None) -> torch.Tensor:
+    if slots.dim() != 1 or slots.dtype not in (torch.int32, torch.int64) or (tokens is not None and slots.shape[0] != tokens):
+        raise ValueError(f"{who}: slots must be a 1-D int32 or int64 tensor, one for each token, got {tuple(slots.shape)} of {slots.dtype}")
+    return slots.contiguous()
+
+
+def _heads_of(t: torch.Tensor) -> torch.Tensor:
+    """[tokens, heads, dim] with the elements of a head contiguous; other strides stay as they are."""
+    return t if t.stride(2) == 1 else t.contiguous()
+
+
+def _kv4_write_impl(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor, k: torch.Tensor,
+                    v: torch.Tensor, slots: torch.Tensor) -> None:
+    _require_cuda(k_codes, k_scales, v_codes, v_scales, k, v, slots)
+    pages, heads, page, d = _check_cache("kv4_write", k_codes, k_scales, v_codes, v_scales)
+    if k.dtype not in (torch.float16, torch.bfloat16, torch.float32) or v.dtype != k.dtype:
+        raise TypeError(f"kv4_write expects k and v of one dtype out of float16, bfloat16, float32; got {k.dtype} and {v.dtype}")
+    if k.dim() != 3 or k.shape[1:] != (heads, d) or v.shape != k.shape:
+        raise ValueError(f"kv4_write: k and v must be [tokens, {heads}, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    tokens = k.shape[0]
+    slots = _check_slots("kv4_write", slots, tokens)
+    _one_device("kv4_write", k_codes, k_scales, v_codes, v_scales, k, v, slots)
+    if tokens == 0:
+        return
+    k, v, dev = _heads_of(k), _heads_of(v), k.device
+    with _on(dev):
+        rc = _lib.load().hx_kv4_write(k.data_ptr(), v.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+                                      v_scales.data_ptr(), slots.data_ptr(), int(slots.dtype == torch.int64), tokens, heads, d, pages,
+                                      page, k.stride(0), k.stride(1), v.stride(0), v.stride(1), _DT[k.dtype], _stream_ptr(dev))
+    _lib.check(rc, "hx_kv4_write")
+
+
+kv4_write_op = torch.library.custom_op("helion_amd::kv4_write", mutates_args=("k_codes", "k_scales", "v_codes", "v_scales"))(_kv4_write_impl)
+
+
+@kv4_write_op.register_fake
+def _(k_codes, k_scales, v_codes, v_scales, k, v, slots):
+    return None
+
+
+def _kv4_read_impl(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor, slots: torch.Tensor,
+                   dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    _require_cuda(k_codes, k_scales, v_codes, v_scales, slots)
+    pages, heads, page, d = _check_cache("kv4_read", k_codes, k_scales, v_codes, v_scales)
+    if dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TypeError(f"kv4_read: dtype must be float16, bfloat16 or float32, got {dtype}")
+    slots = _check_slots("kv4_read", slots)
+    _one_device("kv4_read", k_codes, k_scales, v_codes, v_scales, slots)
+    tokens, dev = slots.shape[0], k_codes.device
+    k = torch.empty((tokens, heads, d), dtype=dtype, device=dev)
+    v = torch.empty((tokens, heads, d), dtype=dtype, device=dev)
+    if tokens:
+        with _on(dev):
+            rc = _lib.load().hx_kv4_read(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
+                                         slots.data_ptr(), int(slots.dtype == torch.int64), k.data_ptr(), v.data_ptr(), tokens, heads, d,
+                                         pages, page, _DT[dtype], _stream_ptr(dev))
+        _lib.check(rc, "hx_kv4_read")
+    return k, v
+
+
+kv4_read_op = torch.library.custom_op("helion_amd::kv4_read", mutates_args=())(_kv4_read_impl)
+
+
+@kv4_read_op.register_fake
+def _(k_codes, k_scales, v_codes, v_scales, slots, dtype):
+    shape = (slots.shape[0], k_codes.shape[1], 2 * k_codes.shape[3])
+    return k_codes.new_empty(shape, dtype=dtype), k_codes.new_empty(shape, dtype=dtype)
+
+
+# ------------------------------------------------------------------------------ attention over it
+def _kv4_attention_into(out: torch.Tensor, q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
+                        v_scales: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, query_start: torch.Tensor | None,
+                        max_query_len: int, scale: float, causal: bool) -> None:
+    _require_cuda(out, q, k_codes, k_scales, v_codes, v_scales, block_table, seq_lens, query_start)
+    pages, kv_heads, page, d = _check_cache("kv4_attention", k_codes, k_scales, v_codes, v_scales)
+    if q.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TypeError(f"kv4_attention expects a float16, bfloat16 or float32 q, got {q.dtype}")
+    if q.dim() != 3 or q.shape[2] != d or kv_heads < 1 or q.shape[1] % kv_heads:
+        raise ValueError(f"kv4_attention: q must be [tokens, a multiple of {kv_heads} heads, {d}], got {tuple(q.shape)}")
+    tokens, heads, _ = q.shape
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32 or seq_lens.dim() != 1:
+        raise ValueError("kv4_attention: block_table must be [sequences, pages] and seq_lens [sequences], both int32")
+    batch, width = block_table.shape
+    if seq_lens.shape[0] != batch:
+        raise ValueError(f"kv4_attention: {seq_lens.shape[0]} lengths for {batch} rows of the block table")
+    if query_start is not None and (query_start.dtype != torch.int32 or query_start.shape != (batch + 1,)):
+        raise ValueError(f"kv4_attention: query_start must be [{batch + 1}] int32, got {tuple(query_start.shape)} of {query_start.dtype}")
+    if query_start is None and tokens != batch:
+        raise ValueError(f"kv4_attention: without query_start q holds one token for each of the {batch} sequences, got {tokens}")
+    if max_query_len < 1:
+        raise ValueError(f"kv4_attention: max_query_len must be at least 1, got {max_query_len}")
+    if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError(f"kv4_attention: out must be contiguous {tuple(q.shape)} of {q.dtype}")
+    _one_device("kv4_attention", out, q, k_codes, k_scales, v_codes, v_scales, block_table, seq_lens, query_start)
+    if tokens == 0 or heads == 0 or batch == 0:
+        return
+    q, dev = _heads_of(q), q.device
+    if width > 1 and block_table.stride(1) != 1 or batch > 1 and block_table.stride(0) < width:
+        block_table = block_table.contiguous()
+    seq_lens = seq_lens.contiguous()
+    query_start = query_start.contiguous() if query_start is not None else None
+    lib = _lib.load()
+    with _on(dev):
+        ws_bytes = lib.hx_kv4_attention_workspace_bytes(tokens, batch, heads, kv_heads, d, page, width,
+                                                        max_query_len if query_start is not None else 1, _DT[q.dtype])
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        rc = lib.hx_kv4_attention(q.data_ptr(), q.stride(0), q.stride(1), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+                                  v_scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr(),
+                                  query_start.data_ptr() if query_start is not None else None, out.data_ptr(), tokens, batch, heads,
+                                  kv_heads, d, pages, page, width, max_query_len, scale, int(causal), _DT[q.dtype],
+                                  ws.data_ptr() if ws is not None else None, ws_bytes, _stream_ptr(dev))
+    _lib.check(rc, "hx_kv4_attention")
+
+
+kv4_attention_out_op = torch.library.custom_op("helion_amd::kv4_attention_out", mutates_args=("out",))(_kv4_attention_into)
+
+
+@kv4_attention_out_op.register_fake
+def _(out, q, k_codes, k_scales, v_codes, v_scales, block_table, seq_lens, query_start, max_query_len, scale, causal):
+    return None
+
+
+def _kv4_attention_impl(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor,
+                        block_table: torch.Tensor, seq_lens: torch.Tensor, query_start: torch.Tensor | None, max_query_len: int,
+                        scale: float, causal: bool) -> torch.Tensor:
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _kv4_attention_into(out, q, k_codes, k_scales, v_codes, v_scales, block_table, seq_lens, query_start, max_query_len, scale, causal)
+    return out
+
+
+kv4_attention_op = torch.library.custom_op("helion_amd::kv4_attention", mutates_args=())(_kv4_attention_impl)
+
+
+@kv4_attention_op.register_fake
+def _(q, k_codes, k_scales, v_codes, v_scales, block_table, seq_lens, query_start, max_query_len, scale, causal):
+    return q.new_empty(q.shape)
+
+
 # ------------------------------------------------------------------------------ what the Python entry points call
 def _caller(impl, op):
     def call(*args):
@@ -411,3 +739,11 @@ cast_e4m3_x3_call = _caller(_cast_e4m3_x3_impl, cast_e4m3_x3_op)
 fp8_quantize_call = _caller(_fp8_quantize_impl, fp8_quantize_op)
 matmul_call = _caller(_matmul_impl, matmul_op)
 attention_call = _caller(_attention_impl, attention_op)
+rms_norm_int8_call = _caller(_rms_norm_int8_impl, rms_norm_int8_op)
+add_rms_norm_int8_call = _caller(_add_rms_norm_int8_impl, add_rms_norm_int8_op)
+int8_quantize_call = _caller(_int8_quantize_impl, int8_quantize_op)
+int8_gemm_call = _caller(_int8_gemm_impl, int8_gemm_op)
+kv4_write_call = _caller(_kv4_write_impl, kv4_write_op)
+kv4_read_call = _caller(_kv4_read_impl, kv4_read_op)
+kv4_attention_call = _caller(_kv4_attention_impl, kv4_attention_op)
+kv4_attention_out_call = _caller(_kv4_attention_into, kv4_attention_out_op)

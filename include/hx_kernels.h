@@ -274,6 +274,75 @@ int hx_attention(const void* q, const void* k, const void* v, void* out, int64_t
 int hx_attention_path(int64_t BH, int64_t M, int64_t N, int64_t D, int dtype, const void* q, const void* k, const void* v,
                       const void* out);
 
+/* ---- Operators of a transformer layer served in few bits (no counterpart in the reference) ---------------------------- */
+
+/* Row-wise quantisation to 8-bit integers, behind a root-mean-square norm or by itself:
+ *   hx_rms_norm_int8:            h = round_T(x + residual) (h = x without a residual);
+ *                                y = h * rsqrt(mean(h^2) + eps) * weight, in fp32
+ *   hx_int8_quantize_per_token:  y = x
+ *   both: scale[row] = max|y| / 127 (1 for a row of zeros), q = y * 127 / max|y| to the nearest integer, ties to even.
+ * A row whose y holds a NaN or an infinity gets that as its scale and zeros as its integers (0 * scale is NaN).
+ * x, residual: rows x width of `dtype` (HX_F16 / HX_BF16 / HX_F32), elements of a row contiguous, row strides in elements;
+ * weight [width] of the same dtype; h_out (with a residual), q and scale are contiguous.  1 <= width <= 65536, any rows,
+ * pointers aligned to their elements.  One launch, no workspace. */
+int hx_rms_norm_int8(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight, float eps,
+                     void* h_out, void* q, float* scale, int64_t rows, int64_t width, int dtype, void* stream);
+int hx_int8_quantize_per_token(const void* x, int64_t x_stride, void* q, float* scale, int64_t rows, int64_t width, int dtype,
+                               void* stream);
+
+/* Product of 8-bit integers with a scale for each row of a and each column of b:
+ *   c[m,n] = cast( (sum_k a[m,k] * b[k,n]) * scale_a[m] * scale_b[n] + bias[n] )
+ * The sum is exact (32-bit integers; K <= 131071, all 256 values of an operand allowed), the rest fp32.  a: rows of K
+ * contiguous bytes, row stride lda >= K; b addressed as b[k*ldb_k + n*ldb_n], strides >= 1; bias [N] of bias_dtype or NULL;
+ * out_dtype HX_F16 / HX_BF16 / HX_F32, row stride ldc.  Any M, N and K >= 1 below 4 GB per operand.  b with ldb_k == 1
+ * (the [N][K] weight of a linear layer), K % 16 == 0 and 16-byte aligned rows is read in place, everything else is copied
+ * into the workspace first; K % 128 != 0 copies a.  workspace: hx_int8_gemm_workspace_bytes(...) bytes (copies, and the
+ * integer sums of a split K), 256-byte aligned. */
+int hx_int8_gemm(const void* a, const void* b, void* c, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb_k, int64_t ldb_n,
+                 int64_t ldc, const float* scale_a, const float* scale_b, const void* bias, int bias_dtype, int out_dtype,
+                 void* workspace, size_t workspace_bytes, void* stream);
+size_t hx_int8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb_k, int64_t ldb_n, const void* a,
+                                    const void* b);
+
+/* A key/value cache held in 4 bits (the open MXFP4 format: e2m1 elements, a power-of-two scale for each 32 of a head).
+ * D = 64, 128 or 256; pages of `page` tokens, a power of two from 16 to 1024; slot = page index * page + place in it.
+ *   k_codes  [pages][heads][page][D/2]            byte b of a token: elements 2b (low half) and 2b+1
+ *   k_scales [pages][heads][page][D/32]           E + 127, E = floor(log2 max|x|) - 2 clamped to -126 .. 125; 255 stands for
+ *                                                 NaN (a block with an infinity or a NaN)
+ *   v_codes  [pages][heads][page/4][16][4][D/32]  piece r of a token: its elements r*D/16 .. ; four tokens side by side
+ *   v_scales [pages][heads][page/4][D/32][4]
+ * each 16-byte aligned.  An element is the e2m1 value nearest to x / 2^E, ties to the even code, at most 6 in magnitude.
+ *
+ * hx_kv4_write: k, v [tokens][heads][D] of `dtype` (HX_F16 / HX_BF16 / HX_F32), elements of a head contiguous, token and head
+ * strides in elements; slots: tokens int32 or int64 values.  A token whose slot lies outside 0 .. pages*page-1 (-1 for
+ * padding) is not written; of several tokens with the same slot the last one is.  One launch, no workspace.
+ * hx_kv4_read: the values at the slots into k, v [tokens][heads][D], contiguous and 16-byte aligned, rounded to `dtype`;
+ * zeros for a slot outside. */
+int hx_kv4_write(const void* k, const void* v, void* k_codes, void* k_scales, void* v_codes, void* v_scales, const void* slots,
+                 int slots_are_int64, int64_t tokens, int64_t heads, int64_t D, int64_t pages, int64_t page, int64_t k_token_stride,
+                 int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, int dtype, void* stream);
+int hx_kv4_read(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, const void* slots,
+                int slots_are_int64, void* k, void* v, int64_t tokens, int64_t heads, int64_t D, int64_t pages, int64_t page, int dtype,
+                void* stream);
+
+/* Attention of new tokens over that cache.  Sequence b has seq_lens[b] keys (the new tokens' own among them), in the pages
+ * block_table[b * table_stride + 0 ..]; its new tokens are rows query_start[b] .. query_start[b+1]-1 of q and out, or row b
+ * alone when query_start is NULL (then tokens == batch).  Query head hq reads key/value head hq / (heads / kv_heads).
+ *   out = softmax(scale * q k^T) v;  causal: new token i of n sees the keys up to seq_lens[b] - n + i, else all of them.
+ * A row that sees no key gives zeros.  Rows of q outside every sequence are neither read nor written.  Table entries behind
+ * the last page of a sequence are not used; the keys of a page that does not exist are masked, as are lengths beyond the table.
+ * q [tokens][heads][D] of `dtype`, elements of a head contiguous, token and head strides in elements; out contiguous,
+ * 16-byte aligned, same dtype.  max_query: the most new tokens of one sequence (sizes the launch; more are computed too,
+ * only slower).  Products of exact bf16 terms (1 for a bf16 q, 2 for fp16, 3 for fp32), fp32 sums and statistics.
+ * workspace: hx_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned (0 where the keys are not split). */
+int hx_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_codes, const void* k_scales,
+                     const void* v_codes, const void* v_scales, const int32_t* block_table, int64_t table_stride,
+                     const int32_t* seq_lens, const int32_t* query_start, void* out, int64_t tokens, int64_t batch, int64_t heads,
+                     int64_t kv_heads, int64_t D, int64_t pages, int64_t page, int64_t table_width, int64_t max_query, float scale,
+                     int causal, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t hx_kv4_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t page,
+                                        int64_t table_width, int64_t max_query, int dtype);
+
 /* ---- Diagnostics (not part of the drop-in interface; no counterpart in the reference) --------------------------------
  * One wave that measures the engine clock of the XCD it lands on as (shader-clock counter delta) / (100 MHz counter
  * delta) over `ticks_100mhz` ticks of the latter (at most 10000 = 100 us; the wave sleeps 3-4 us between two readings of

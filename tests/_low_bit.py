@@ -1,0 +1,112 @@
+"""Inputs and checks shared by the CPU and GPU tests of the low-bit serving operators."""
+from __future__ import annotations
+
+import torch
+
+from oracle import low_bit as ref
+
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def norm_inputs(rows, width, dtype, residual, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, width, generator=g).to(dtype)
+    r = (3 * torch.randn(rows, width, generator=g)).to(dtype) if residual else None
+    w = (1 + 0.3 * torch.randn(width, generator=g)).to(dtype)
+    if rows > 2:
+        x[1] = 0
+        if residual:
+            r[1] = 0
+    return x, r, w
+
+
+def check_rows(q, scale, y, roundings):
+    """q, scale against the float64 values y: integers are within half a step and the fp32 roundings of y / scale"""
+    want = ref.row_scale(y)
+    assert scale.dtype == F32 and scale.shape == (*y.shape[:-1], 1)
+    assert ((scale.double() - want).abs() <= (roundings + 2) * 2.0**-24 * want).all()
+    steps = torch.where(y.abs().amax(-1, keepdim=True) == 0, torch.zeros_like(y), y / want)
+    assert q.dtype == torch.int8
+    assert ((q.double() - steps).abs() <= 0.5 + 127 * roundings * 2.0**-24).all()
+    assert (q.int().abs() <= 127).all()
+
+
+def gemm_inputs(m, n, k, seed, bias=None, layout="col"):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8)
+    y = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8).t()
+    if layout == "row":
+        y = y.contiguous()
+    sa = torch.exp(torch.randn(m, 1, generator=g)) * 0.01
+    sb = torch.exp(torch.randn(1, n, generator=g)) * 0.001
+    b = torch.randn(n, generator=g).to(bias) if bias is not None else None
+    return x, y, sa, sb, b
+
+
+def check_gemm(out, x, y, sa, sb, b, out_dtype):
+    want, size = ref.int8_gemm(x, y, sa, sb, b)
+    assert out.dtype == out_dtype and out.shape == want.shape
+    # the integer to fp32, two scales, the bias
+    err, most = (out.double() - want).abs(), ref.float_bound(want, size, out_dtype, 4)
+    assert (err <= most).all(), f"off by up to {float((err / most).max()):.2f} of the bound"
+
+
+def attention_case(dtype, dim, page, kv_heads, group, lens, news=None, seed=0, spare=2):
+    """A filled cache in pages of any order, garbage where no key is, tables with entries that are not to be used."""
+    g = torch.Generator().manual_seed(seed)
+    need = [-(-n // page) for n in lens]
+    pages, width = sum(need) + spare, max(max(need), 1) + 1
+    k = torch.randn(pages, kv_heads, page, dim, generator=g)
+    v = torch.randn(pages, kv_heads, page, dim, generator=g)
+    kc, ks = ref.encode(k)
+    vc, vs = ref.encode(v)
+    order = torch.randperm(pages, generator=g).tolist()
+    table = torch.full((len(lens), width), -7, dtype=torch.int32)
+    at = 0
+    used = torch.zeros(pages, page, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        for i in range(need[b]):
+            table[b, i] = order[at]
+            used[order[at], : min(page, n - i * page)] = True
+            at += 1
+    # what nobody has written: NaN scales, any codes
+    gone = ~used[:, None, :, None].expand(pages, kv_heads, page, dim // 32)
+    ks = torch.where(gone, torch.full_like(ks, 255), ks)
+    vs = torch.where(gone, torch.full_like(vs, 255), vs)
+    tokens = sum(news) if news is not None else len(lens)
+    q = (1.5 * torch.randn(tokens, kv_heads * group, dim, generator=g)).to(dtype)
+    start = torch.tensor([0] + news).cumsum(0).int() if news is not None else None
+    cache = (*ref.to_layout(kc, ks, False), *ref.to_layout(vc, vs, True))
+    return q, cache, table, torch.tensor(lens, dtype=torch.int32), start
+
+
+def check_attention(out, q, cache, table, lens, start, scale=None, causal=True, p_terms=2, rows=None):
+    want, size, spread = ref.attention(q, *cache, table, lens, start, scale, causal)
+    most = ref.attention_bound(want, size, spread, q.dtype, int(lens.max()) if lens.numel() else 0, q.shape[2], p_terms)
+    got = out.double()
+    if rows is not None:
+        got, want, most = got[rows], want[rows], most[rows]
+    assert torch.equal(got.isnan(), want.isnan())
+    err = torch.where(want.isnan(), torch.zeros_like(got), (got - want).abs())
+    most = torch.where(want.isnan(), torch.ones_like(most), most)
+    assert (err <= most).all(), f"off by up to {float((err / most).max()):.2f} of the bound"
+
+
+def p_terms(dtype):
+    return 3 if dtype == F32 else 2
+
+
+# (dtype, dim, page, kv_heads, group, lens, new tokens or None)
+ATTENTION = [
+    (BF, 128, 16, 2, 4, [1], None),
+    (BF, 128, 64, 1, 8, [33, 0, 16, 65], None),             # an empty sequence, a whole block, one past it
+    (HF, 64, 16, 3, 1, [31, 32, 100], None),
+    (F32, 128, 32, 1, 5, [70], None),
+    (BF, 256, 16, 1, 2, [40, 17], None),
+    (HF, 256, 32, 1, 3, [35], [3]),
+    (HF, 128, 16, 1, 7, [50, 20], [3, 20]),                  # a piece of a prompt and a whole one, 60 rows and 140
+    (BF, 64, 128, 2, 2, [40, 1, 0, 9], [12, 1, 0, 4]),
+    (F32, 64, 16, 1, 2, [30, 5], [9, 5]),
+    (BF, 128, 32, 1, 16, [90], [5]),                         # more than 16 rows
+    (HF, 64, 16, 1, 3, [25], [25]),
+]

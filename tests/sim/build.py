@@ -27,7 +27,7 @@ BUILD = SIM / "_build"
 LIB = SIM / "libhx_sim.so"
 CXX = "/opt/rocm/llvm/bin/clang++"
 UNITS = ["hx_common.cpp", "fp8_gemm.hip", "fp8_attention.hip", "moe_gemm.hip", "moe_routing.hip", "fp8_quantize.hip",
-         "matmul16.hip", "attention16.hip", "diag.hip"]
+         "matmul16.hip", "attention16.hip", "norm_int8.hip", "int8_gemm.hip", "kv4_cache.hip", "kv4_attention.hip", "diag.hip"]
 FLAGS = ["-std=c++17", "-O1", "-g", "-fPIC", "-fno-strict-aliasing", "-ffp-contract=off", "-Wno-unknown-attributes",
          "-Wno-unused-value", "-Wno-builtin-macro-redefined", "-Wno-reserved-macro-identifier", "-Wno-macro-redefined",
          "-Wno-ignored-attributes", "-Wno-pass-failed", "-Wno-unknown-pragmas", "-fno-stack-protector", "-mf16c"]

@@ -87,10 +87,12 @@ void ds_read_tr(int elem_bytes, const void* lds_ptr, void* out8, int site);
 void dma(const void* gptr, uint32_t lds_dst, int bytes);
 uint32_t lds_addr(const void* p);
 int cvt_pk_fp8(float a, float b, int old, bool hi);
+float cvt_f32_fp4(uint32_t code, float scale);           // e2m1 times 2^(exponent field of scale - 127)
+uint32_t cvt_fp4_f32(float f, float scale);              // to nearest, ties to the even code, at most 6
 float cvt_f32_fp8(int v, int sel);
 uint64_t clock100mhz();
 
-enum { MFMA_F8_32x32x64 = 0, MFMA_F8_16x16x128, MFMA_F8_16x16x32, MFMA_BF16_32x32x16, MFMA_F16_32x32x16, MFMA_BF16_16x16x32, MFMA_F16_16x16x32 };
+enum { MFMA_F8_32x32x64 = 0, MFMA_F8_16x16x128, MFMA_F8_16x16x32, MFMA_BF16_32x32x16, MFMA_F16_32x32x16, MFMA_BF16_16x16x32, MFMA_F16_16x16x32, MFMA_I8_16x16x64 };
 
 // runs `fn` once per work-item of the grid; returns hipSuccess or hipErrorLaunchFailure (message: hx_sim_last_fault)
 hipError_t run(dim3 grid, dim3 block, const std::function<void()>& fn, const void* kernel);
@@ -111,6 +113,9 @@ typedef short hxs_v4s __attribute__((ext_vector_type(4)));
 typedef __bf16 hxs_v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 hxs_v8h __attribute__((ext_vector_type(8)));
 typedef unsigned hxs_v2u __attribute__((ext_vector_type(2)));
+typedef int hxs_v4i __attribute__((ext_vector_type(4)));
+typedef float hxs_v2f __attribute__((ext_vector_type(2)));
+typedef __bf16 hxs_v2bf __attribute__((ext_vector_type(2)));
 
 namespace hxsim {
 template <int KIND, typename AB, typename CD>
@@ -133,6 +138,24 @@ inline hxs_v2u permlane32_swap(uint32_t a, uint32_t b, int site) {
   uint32_t o[2];
   permlane32_swap_u32(a, b, o, site);
   return (hxs_v2u){o[0], o[1]};
+}
+inline hxs_v2f cvt_pk_f32_fp4(uint32_t src, float scale, int sel) {
+  const uint32_t b = src >> (8 * sel);
+  return (hxs_v2f){cvt_f32_fp4(b & 15, scale), cvt_f32_fp4((b >> 4) & 15, scale)};
+}
+inline hxs_v2bf cvt_pk_bf16_fp4(uint32_t src, float scale, int sel) {
+  const hxs_v2f f = cvt_pk_f32_fp4(src, scale, sel);
+  return (hxs_v2bf){(__bf16)f[0], (__bf16)f[1]};
+}
+inline uint32_t cvt_pk_fp4_f32(uint32_t old, float a, float b, float scale, int sel) {
+  const uint32_t pair = cvt_fp4_f32(a, scale) | (cvt_fp4_f32(b, scale) << 4);
+  return (old & ~(255u << (8 * sel))) | (pair << (8 * sel));
+}
+inline uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {  // selectors 0 .. 7 only
+  const uint64_t both = ((uint64_t)hi << 32) | lo;
+  uint32_t r = 0;
+  for (int i = 0; i < 4; ++i) r |= (uint32_t)((both >> (8 * ((sel >> (8 * i)) & 7))) & 255) << (8 * i);
+  return r;
 }
 template <typename T>
 inline T mov_dpp(T v, int ctrl, int rm, int bm, bool bc, int site) {
@@ -181,6 +204,11 @@ inline T shfl_xor(T v, int mask, int site) {
 #define __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, x, y, z) hxsim::mfma_t<hxsim::MFMA_F16_16x16x32, hxs_v8h, hxs_v4f>((a), (b), (c), __LINE__)
 #define __builtin_amdgcn_ds_read_tr8_b64_v2i32(p) hxsim::ds_read_tr8_b64((const void*)(uintptr_t)(p), __LINE__)
 #define __builtin_amdgcn_ds_read_tr16_b64_v4i16(p) hxsim::ds_read_tr16_b64((const void*)(uintptr_t)(p), __LINE__)
+#define __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, x, y, z) hxsim::mfma_t<hxsim::MFMA_I8_16x16x64, hxs_v4i, hxs_v4i>((a), (b), (c), __LINE__)
+#define __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(src, scale, sel) hxsim::cvt_pk_f32_fp4((src), (scale), (sel))
+#define __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(src, scale, sel) hxsim::cvt_pk_bf16_fp4((src), (scale), (sel))
+#define __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(old, a, b, scale, sel) hxsim::cvt_pk_fp4_f32((old), (a), (b), (scale), (sel))
+#define __builtin_amdgcn_perm(hi, lo, sel) hxsim::perm((hi), (lo), (sel))
 #define __builtin_amdgcn_cvt_pk_fp8_f32(a, b, old, hi) hxsim::cvt_pk_fp8((a), (b), (old), (hi))
 #define __builtin_amdgcn_cvt_f32_fp8(v, sel) hxsim::cvt_f32_fp8((v), (sel))
 
@@ -209,6 +237,12 @@ template <typename T>
 HXSIM_UNTRACED inline T atomicMax(T* p, T v) {
   const T old = *p;
   if (v > old) *p = v;
+  return old;
+}
+template <typename T>
+HXSIM_UNTRACED inline T atomicOr(T* p, T v) {
+  const T old = *p;
+  *p = old | v;
   return old;
 }
 template <typename T>

@@ -210,3 +210,106 @@ def attention16(q, k, v, scale_dim=None, end_flush=True, want_path=None):
         rc = lib.hx_attention(Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), bh, m, n, d, scale_dim or d, _DT[q.dtype], None)
         simlib.check(rc, "hx_attention")
         return O.clone()
+
+
+def _rows_in(ar, x, stride):
+    """x [rows, width] in a guarded buffer, `stride` elements from row to row"""
+    if stride is None or stride == x.shape[1]:
+        return ar.put(x), x.shape[1]
+    buf = torch.zeros(x.shape[0], stride, dtype=x.dtype)
+    buf[:, : x.shape[1]] = x
+    flat = buf.reshape(-1)[: (x.shape[0] - 1) * stride + x.shape[1]]  # nothing behind the last row's last element
+    return ar.put(flat), stride
+
+
+def rms_norm_int8(x, weight=None, residual=None, eps=1e-6, stride=None, end_flush=True):
+    """(q, scale, h); weight None: plain quantisation"""
+    lib = simlib.load()
+    rows, width = x.shape
+    with simlib.Arena(end_flush) as ar:
+        X, xs = _rows_in(ar, x, stride)
+        Q, S = ar.out((rows, width), torch.int8), ar.out((rows, 1), torch.float32)
+        if weight is None:
+            rc = lib.hx_int8_quantize_per_token(X.data_ptr(), xs, Q.data_ptr(), S.data_ptr(), rows, width, _DT[x.dtype], None)
+            simlib.check(rc, "hx_int8_quantize_per_token")
+            return Q.clone(), S.clone(), None
+        R, rs = _rows_in(ar, residual, stride) if residual is not None else (None, 0)
+        W = ar.put(weight)
+        H = ar.out((rows, width), x.dtype) if residual is not None else None
+        rc = lib.hx_rms_norm_int8(X.data_ptr(), xs, _p(R), rs, W.data_ptr(), eps, _p(H), Q.data_ptr(), S.data_ptr(), rows, width,
+                                  _DT[x.dtype], None)
+        simlib.check(rc, "hx_rms_norm_int8")
+        return Q.clone(), S.clone(), H.clone() if H is not None else None
+
+
+def int8_gemm(x, y, scale_a, scale_b, bias=None, out_dtype=torch.bfloat16, end_flush=True):
+    lib = simlib.load()
+    m, k = x.shape
+    n = y.shape[1]
+    with simlib.Arena(end_flush) as ar:
+        X = ar.put(x)
+        if y.stride(0) == 1:
+            Y, ldb_k, ldb_n = ar.put(y.t()), 1, k
+        else:
+            Y, ldb_k, ldb_n = ar.put(y), n, 1
+        C = ar.out((m, n), out_dtype, fill=0xFF)
+        A, B = ar.put(scale_a), ar.put(scale_b)
+        bb = ar.put(bias) if bias is not None else None
+        wsb = lib.hx_int8_gemm_workspace_bytes(m, n, k, k, ldb_k, ldb_n, X.data_ptr(), Y.data_ptr())
+        ws = None
+        if wsb:  # 256-byte aligned, nothing behind it
+            raw = ar.empty((wsb + 255) // 256 * 256)
+            ws = raw
+        rc = lib.hx_int8_gemm(X.data_ptr(), Y.data_ptr(), C.data_ptr(), m, n, k, k, ldb_k, ldb_n, n, A.data_ptr(), B.data_ptr(), _p(bb),
+                              _DT[bias.dtype] if bias is not None else 0, _DT[out_dtype], _p(ws), wsb, None)
+        simlib.check(rc, "hx_int8_gemm")
+        return C.clone()
+
+
+def kv4_write(cache, k, v, slots, end_flush=True):
+    """writes into clones of the cache's four tensors and returns them"""
+    lib = simlib.load()
+    pages, heads, page, half = cache[0].shape
+    with simlib.Arena(end_flush) as ar:
+        c = [ar.put(t) for t in cache]
+        span = lambda t: t.as_strided((1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())),), (1,), t.storage_offset())
+        K, V, S = ar.put(span(k)), ar.put(span(v)), ar.put(slots)
+        rc = lib.hx_kv4_write(K.data_ptr(), V.data_ptr(), *(t.data_ptr() for t in c), S.data_ptr(), int(slots.dtype == torch.int64),
+                              k.shape[0], heads, 2 * half, pages, page, k.stride(0), k.stride(1), v.stride(0), v.stride(1), _DT[k.dtype], None)
+        simlib.check(rc, "hx_kv4_write")
+        return [t.clone() for t in c]
+
+
+def kv4_read(cache, slots, dtype, end_flush=True):
+    lib = simlib.load()
+    pages, heads, page, half = cache[0].shape
+    with simlib.Arena(end_flush) as ar:
+        c = [ar.put(t) for t in cache]
+        S = ar.put(slots)
+        K = ar.out((slots.shape[0], heads, 2 * half), dtype, fill=0xFF)
+        V = ar.out((slots.shape[0], heads, 2 * half), dtype, fill=0xFF)
+        rc = lib.hx_kv4_read(*(t.data_ptr() for t in c), S.data_ptr(), int(slots.dtype == torch.int64), K.data_ptr(), V.data_ptr(),
+                             slots.shape[0], heads, 2 * half, pages, page, _DT[dtype], None)
+        simlib.check(rc, "hx_kv4_read")
+        return K.clone(), V.clone()
+
+
+def kv4_attention(q, cache, table, lens, start=None, max_query=None, scale=None, causal=True, end_flush=True, fill=0):
+    lib = simlib.load()
+    pages, kv_heads, page, half = cache[0].shape
+    tokens, heads, d = q.shape
+    batch, width = table.shape
+    if max_query is None:
+        max_query = 1 if start is None else max(1, int((start[1:] - start[:-1]).max()))
+    with simlib.Arena(end_flush) as ar:
+        c = [ar.put(t) for t in cache]
+        Q, T, L = ar.put(q), ar.put(table), ar.put(lens)
+        S = ar.put(start) if start is not None else None
+        O = ar.out(q.shape, q.dtype, fill=fill)
+        wsb = lib.hx_kv4_attention_workspace_bytes(tokens, batch, heads, kv_heads, d, page, width, max_query, _DT[q.dtype])
+        ws = ar.empty(wsb) if wsb else None
+        rc = lib.hx_kv4_attention(Q.data_ptr(), heads * d, d, *(t.data_ptr() for t in c), T.data_ptr(), width, L.data_ptr(), _p(S),
+                                  O.data_ptr(), tokens, batch, heads, kv_heads, d, pages, page, width, max_query,
+                                  d**-0.5 if scale is None else scale, int(causal), _DT[q.dtype], _p(ws), wsb, None)
+        simlib.check(rc, "hx_kv4_attention")
+        return O.clone()
