@@ -23,6 +23,8 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 
 #define HX_LDS(p) ((__attribute__((address_space(3))) void*)(p))
+// memory that no kernel in flight writes, read at a wave-uniform address: the compiler then uses scalar loads
+#define HX_CONSTANT(T, p) ((const __attribute__((address_space(4))) T*)(p))
 #define HX_GLB(p) ((const __attribute__((address_space(1))) void*)(p))
 
 // 16-byte global->LDS DMA: every lane supplies its own global address; the wave writes 1024

@@ -24,6 +24,7 @@
 #include <type_traits>
 
 #define KA_M0 (-3e38f)  // the reference point of a row that has seen no key
+#define KA_PIECE 1024  // keys of a split at least
 #define KA_STEP 8.f     // it moves only when a score lies 2^8 above it: p stays below 256, and few tiles rescale O
 
 int kv4_check_cache(const char* who, const void* kc, const void* ks, const void* vc, const void* vs, int64_t pages, int64_t page,
@@ -39,8 +40,8 @@ struct KaArgs {
   const int *seq_lens, *query_start;
   float* part_o;   // [tokens * heads][splits][D]
   float* part_ml;  // [tokens * heads][splits][2]
-  float c;         // softmax scale * log2(e)
-  int tokens, batch, heads, kv_heads, pages, page_shift, table_width, causal, splits, blocks;
+  float c;         // |softmax scale| * log2(e); a negative scale turns the queries around instead
+  int tokens, batch, heads, kv_heads, pages, page_shift, table_width, causal, splits, blocks, negate;
 };
 
 template <int DT>
@@ -58,6 +59,9 @@ struct KaT<HX_F32> {
   typedef float T;
 };
 
+// a wave-uniform integer that no kernel writes: through the scalar cache
+__device__ __forceinline__ int ka_scalar(const int* p) { return *HX_CONSTANT(int, p); }
+
 // byte `sel` (a constant once the loops are unrolled) of `codes` as two bf16 in one register
 __device__ __forceinline__ uint32_t ka_pair(uint32_t codes, float scale, int sel) {
   v2bf p;
@@ -70,6 +74,12 @@ __device__ __forceinline__ uint32_t ka_pair(uint32_t codes, float scale, int sel
   return __builtin_bit_cast(uint32_t, p);
 }
 
+// codes that the launch reads once (one block of rows) do not displace what is reused
+template <bool NT, typename V>
+__device__ __forceinline__ V ka_codes(const V* p) {
+  return NT ? __builtin_nontemporal_load(p) : *p;
+}
+
 // f = t[0] + t[1] + .. + t[N-1] with bf16 terms, each the rounding of what the ones before it leave
 template <int N>
 __device__ __forceinline__ void ka_terms(float f, __bf16 (&t)[N]) {
@@ -80,13 +90,15 @@ __device__ __forceinline__ void ka_terms(float f, __bf16 (&t)[N]) {
   }
 }
 
-template <int D, int DT, int NQ, int NP, int RB, int NW>
-__global__ __launch_bounds__(NW * 64) void hx_kv4_attention_kernel(KaArgs a) {
+template <int D, int DT, int NQ, int NP, int RB, int NW, int TB>
+__global__ __launch_bounds__(NW * 64, RB > 1 || D > 128 || DT == HX_F32 ? 2 : D == 64 ? 4 : DT == HX_BF16 ? 3 : 2) void hx_kv4_attention_kernel(KaArgs a) {
   typedef typename KaT<DT>::T T;
+  constexpr bool NT = RB == 1;
   constexpr int DG = D / 4;    // elements of a key per lane
   constexpr int KM = DG / 8;   // MFMAs per 16 keys = dwords of a key per lane
   constexpr int PB = D / 32;   // bytes of a piece = scales of a token = dwords of values per lane and 16 keys
   constexpr int VJ = D / 16;   // MFMAs of the second product
+  constexpr int TK = 16 * TB;  // keys of a tile
   constexpr int OSTR = D + 4;  // row stride of the joining buffer, in floats
   __shared__ __attribute__((aligned(16))) float joint[NW][16][OSTR];
   __shared__ float stat_m[NW][16], stat_l[NW][16];
@@ -102,30 +114,34 @@ __global__ __launch_bounds__(NW * 64) void hx_kv4_attention_kernel(KaArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = a.heads / a.kv_heads;
-  const int start = a.query_start ? a.query_start[b] : b;
-  int n_new = a.query_start ? a.query_start[b + 1] - start : 1;
+  const int start = a.query_start ? ka_scalar(a.query_start + b) : b;
+  int n_new = a.query_start ? ka_scalar(a.query_start + b + 1) - start : 1;
   if (start < 0 || start >= a.tokens) return;
   n_new = min(n_new, a.tokens - start);
   const int pm = (1 << a.page_shift) - 1;
-  const int kv_len = (int)min((long)max(a.seq_lens[b], 0), (long)a.table_width << a.page_shift);
+  const int kv_len = (int)min((long)max(ka_scalar(a.seq_lens + b), 0), (long)a.table_width << a.page_shift);
   const int* table = a.table + b * a.table_stride;
-  const long rows = (long)n_new * G;
+  const int rows = n_new * G;  // (tokens * heads < 2^31, checked by the host)
 
-  for (long block = block0; block * (16 * RB) < rows; block += a.blocks) {
-    const long row0 = block * (16 * RB);
-    const int i_first = (int)(row0 / G), i_last = (int)((min(row0 + 16 * RB, rows) - 1) / G);
+  // where this lane's share of 16 keys lies
+  const uint32_t kc_off = r16 * (D / 2) + g * (DG / 2), vc_off = (g * 16 + r16) * (4 * PB);
+  const uint32_t ks_off = r16 * PB + (D == 64 ? g >> 1 : D == 128 ? g : 2 * g), vs_off = (g * PB + r16 / (512 / D)) * 4;
+
+  for (int row0 = block0 * 16 * RB; row0 < rows; row0 += a.blocks * 16 * RB) {
+    const int i_first = (unsigned)row0 / (unsigned)G, i_last = (unsigned)(min(row0 + 16 * RB, rows) - 1) / (unsigned)G;
     const int see_all = a.causal ? kv_len - n_new + i_first : kv_len - 1;            // last key every row sees
     const int n_keys = a.causal ? max(kv_len - n_new + i_last + 1, 0) : kv_len;      // keys any row sees
-    const int tiles = (n_keys + 31) >> 5;
-    const int t_begin = (int)((long)tiles * split / a.splits), t_end = (int)((long)tiles * (split + 1) / a.splits);
+    const int tiles = (n_keys + TK - 1) / TK;
+    const int piece = max((tiles + a.splits - 1) / a.splits, a.splits > 1 ? KA_PIECE / TK : 1);
+    const int t_begin = min(split * piece, tiles), t_end = min(t_begin + piece, tiles);
 
     // ---- this wave's queries: column c = lane % 16 of block rb is row row0 + 16 rb + c
     v8bf qf[RB][NQ][KM];
     int last[RB];  // the last key the row sees
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      const long row = row0 + 16 * rb + r16;
-      const int i = (int)(min(row, rows - 1) / G), hq = h * G + (int)(min(row, rows - 1) - (long)i * G);
+      const int row = min(row0 + 16 * rb + r16, rows - 1);
+      const int i = (unsigned)row / (unsigned)G, hq = h * G + row - i * G;
       last[rb] = a.causal ? kv_len - n_new + i : kv_len - 1;
       const T* qp = (const T*)a.q + (start + i) * a.q_token_stride + hq * a.q_head_stride + DG * g;
       typedef T Tv __attribute__((ext_vector_type(8), aligned(sizeof(T))));
@@ -135,7 +151,7 @@ __global__ __launch_bounds__(NW * 64) void hx_kv4_attention_kernel(KaArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           __bf16 t[NQ];
-          ka_terms<NQ>((float)raw[e], t);
+          ka_terms<NQ>(a.negate ? -(float)raw[e] : (float)raw[e], t);
 #pragma unroll
           for (int n = 0; n < NQ; ++n) qf[rb][n][m][e] = t[n];
         }
@@ -152,63 +168,62 @@ __global__ __launch_bounds__(NW * 64) void hx_kv4_attention_kernel(KaArgs a) {
       for (int j = 0; j < VJ; ++j) o[rb][j] = (v4f){0.f, 0.f, 0.f, 0.f};
     }
 
-    // ---- a tile on its way: pages first, then codes and scales, one step ahead of their use.  Every load is in range
-    // whatever the tables hold: blocks past the last key are the last block, a page that does not exist is page 0, and
-    // both are masked.
+    // ---- tiles on their way: pages first, then codes and scales.  Every load is in range whatever the tables hold:
+    // blocks past the last key are the last block, a page that does not exist is page 0, and both are masked.
     struct Tile {
-      uint32_t k[2][KM], v[2][PB], ks[2], vs[2];
-      int there;
+      uint32_t k[TB][KM], v[TB][PB], ks[TB], vs[TB];
+      uint32_t nan_at;  // values of this lane (bit 4 tb + i) that are NaN in a tile with a mask
+      uint32_t there;
     };
     const int last_block = (n_keys - 1) >> 4;
-    auto page_of = [&](int t, int tb) { return table[min(2 * t + tb, last_block) >> (a.page_shift - 4)]; };
-    auto load = [&](Tile& x, int t, int page0, int page1) {
+    auto page_of = [&](int t, int tb) { return ka_scalar(table + (min(TB * t + tb, last_block) >> (a.page_shift - 4))); };
+    auto load = [&](Tile& x, int t, const int(&pages)[TB]) {
       x.there = 0;
+      x.nan_at = 0;
 #pragma unroll
-      for (int tb = 0; tb < 2; ++tb) {
-        int page = tb ? page1 : page0;
+      for (int tb = 0; tb < TB; ++tb) {
+        int page = pages[tb];
         const bool ok = (unsigned)page < (unsigned)a.pages;
         page = ok ? page : 0;
-        x.there |= ok << tb;
-        const long at = (((long)page * a.kv_heads + h) << a.page_shift) + ((min(2 * t + tb, last_block) << 4) & pm);
-        const uint8_t* kc = a.kc + at * (D / 2) + r16 * (D / 2) + g * (DG / 2);
-        const uint8_t* vc = a.vc + at * (D / 2) + (g * 16 + r16) * (4 * PB);
+        x.there |= (uint32_t)ok << tb;
+        const long at = (((long)page * a.kv_heads + h) << a.page_shift) + ((min(TB * t + tb, last_block) << 4) & pm);
+        const uint8_t* kc = a.kc + at * (D / 2);  // (uniform bases, 32-bit offsets per lane)
+        const uint8_t* vc = a.vc + at * (D / 2);
         if (KM == 2) {
-          const v2i u = *(const v2i*)kc;
+          const v2i u = ka_codes<NT>((const v2i*)(kc + kc_off));
           x.k[tb][0] = u[0], x.k[tb][1] = u[1];
         } else {
 #pragma unroll
           for (int m = 0; m < KM; m += 4) {
-            const v4i u = *(const v4i*)(kc + 4 * m);
+            const v4i u = ka_codes<NT>((const v4i*)(kc + kc_off + 4 * m));
             x.k[tb][m] = u[0], x.k[tb][m + 1] = u[1], x.k[tb][m + 2] = u[2], x.k[tb][m + 3] = u[3];
           }
         }
+        const uint8_t* ks = a.ks + at * PB;
+        if (D == 256) x.ks[tb] = *(const uint16_t*)(ks + ks_off);
+        else x.ks[tb] = ks[ks_off];
         if (PB == 2) {
-          const v2i u = *(const v2i*)vc;
+          const v2i u = ka_codes<NT>((const v2i*)(vc + vc_off));
           x.v[tb][0] = u[0], x.v[tb][1] = u[1];
         } else {
 #pragma unroll
           for (int m = 0; m < PB; m += 4) {
-            const v4i u = *(const v4i*)(vc + 4 * m);
+            const v4i u = ka_codes<NT>((const v4i*)(vc + vc_off + 4 * m));
             x.v[tb][m] = u[0], x.v[tb][m + 1] = u[1], x.v[tb][m + 2] = u[2], x.v[tb][m + 3] = u[3];
           }
         }
-        const uint8_t* ks = a.ks + at * PB + r16 * PB;
-        if (D == 64) x.ks[tb] = ks[g >> 1];
-        else if (D == 128) x.ks[tb] = ks[g];
-        else x.ks[tb] = *(const uint16_t*)(ks + 2 * g);
-        x.vs[tb] = *(const uint32_t*)(a.vs + at * PB + (g * PB + r16 / (512 / D)) * 4);
+        x.vs[tb] = *(const uint32_t*)(a.vs + at * PB + vs_off);
       }
     };
 
-    auto multiply = [&](const Tile& x, int t) {
-      // scores
-      v4f s[RB][2];
+    v4f s[RB][TB];
+    auto scores = [&](const Tile& x, v4f(&to)[RB][TB]) {
 #pragma unroll
-      for (int tb = 0; tb < 2; ++tb) {
+      for (int tb = 0; tb < TB; ++tb) {
         v8bf kf[KM];
 #pragma unroll
         for (int m = 0; m < KM; ++m) {
-          const float sc = kv4_scale(D == 256 ? (m < KM / 2 ? x.ks[tb] & 255 : x.ks[tb] >> 8) : x.ks[tb]);
+          const float sc = kv4_scale_of(x.ks[tb], D == 256 && m >= KM / 2 ? 1 : 0);
           v4i u;
 #pragma unroll
           for (int e = 0; e < 4; ++e) u[e] = (int)ka_pair(x.k[tb][m], sc, e);
@@ -221,64 +236,83 @@ __global__ __launch_bounds__(NW * 64) void hx_kv4_attention_kernel(KaArgs a) {
           for (int n = NQ - 1; n >= 0; --n)
 #pragma unroll
             for (int m = 0; m < KM; ++m) acc = Mfma16<true>::run16(kf[m], qf[rb][n][m], acc);
-          s[rb][tb] = acc * a.c;
+          to[rb][tb] = acc;
         }
       }
-      uint32_t vs[2] = {x.vs[0], x.vs[1]};
-      uint32_t nan_at = 0;  // values of this lane (bit 4 tb + i) that are NaN in a tile with a mask
-      if (32 * t + 31 > see_all || x.there != 3) {
+    };
+    auto mask = [&](Tile& x, v4f(&to)[RB][TB], int t) {
+      if (TK * t + TK - 1 > see_all || x.there != (1u << TB) - 1) {
+        HX_OPAQUE_V(x.nan_at);  // keeps this a branch: as selects the masks would cost every tile as much as the softmax
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-          for (int tb = 0; tb < 2; ++tb)
+          for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (32 * t + 16 * tb + 4 * g + e > last[rb] || !((x.there >> tb) & 1)) s[rb][tb][e] = -INFINITY;
+              if (TK * t + 16 * tb + 4 * g + e > last[rb] || !((x.there >> tb) & 1)) to[rb][tb][e] = -INFINITY;
         // A masked p is zero, but zero times NaN is not: the scales behind the last key (memory that nobody has written, or
         // another sequence's) become small finite ones, and the NaN that a row does see is put in after the product.
 #pragma unroll
-        for (int tb = 0; tb < 2; ++tb)
+        for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const bool there = 32 * t + 16 * tb + 4 * g + i < n_keys && ((x.there >> tb) & 1);
+            const bool there = TK * t + 16 * tb + 4 * g + i < n_keys && ((x.there >> tb) & 1);
             const bool nan = ((x.vs[tb] >> (8 * i)) & 255) == 255;
-            if (!there || nan) vs[tb] = (vs[tb] & ~(255u << (8 * i))) | (1u << (8 * i));
-            if (there && nan) nan_at |= 1u << (4 * tb + i);
+            if (!there || nan) x.vs[tb] = (x.vs[tb] & ~(255u << (8 * i))) | (1u << (8 * i));
+            if (there && nan) x.nan_at |= 1u << (4 * tb + i);
           }
       }
-      // softmax: the reference point of a row is the same in the four lanes that share its column
-      v8bf pf[RB][NP];
+    };
+    // Moves the reference points where a score lies far above.  The four lanes that share a column agree on its point.
+    auto vote = [&]() {
+      float top[RB];
+      bool far = false;
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
-        float top = fmaxf(fmaxf(fmaxf(s[rb][0][0], s[rb][0][1]), fmaxf(s[rb][0][2], s[rb][0][3])),
-                          fmaxf(fmaxf(s[rb][1][0], s[rb][1][1]), fmaxf(s[rb][1][2], s[rb][1][3])));
-        if (__builtin_amdgcn_ballot_w64(top > mx[rb] + KA_STEP) != 0) {
-          top = fmaxf(top, __shfl_xor(top, 16));
-          top = fmaxf(top, __shfl_xor(top, 32));
-          const float next = fmaxf(mx[rb], top), f = __builtin_amdgcn_exp2f(mx[rb] - next);
+        top[rb] = s[rb][0][0];
+#pragma unroll
+        for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top[rb] = fmaxf(top[rb], s[rb][tb][e]);
+        top[rb] *= a.c;
+        far |= top[rb] > mx[rb] + KA_STEP;
+      }
+      if (__builtin_amdgcn_ballot_w64(far) != 0) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          top[rb] = fmaxf(top[rb], __shfl_xor(top[rb], 16));
+          top[rb] = fmaxf(top[rb], __shfl_xor(top[rb], 32));
+          const float next = top[rb] > mx[rb] + KA_STEP ? top[rb] : mx[rb];
+          const float f = __builtin_amdgcn_exp2f(mx[rb] - next);
           mx[rb] = next;
           l[rb] *= f;
 #pragma unroll
           for (int j = 0; j < VJ; ++j) o[rb][j] *= f;
         }
+      }
+    };
+    auto weights = [&](v8bf(&pf)[RB][NP], int half) {
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
         for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float p = __builtin_amdgcn_exp2f(s[rb][tb][e] - mx[rb]);
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][2 * half + tb][e], a.c, -mx[rb]));
             l[rb] += p;
             __bf16 u[NP];
             ka_terms<NP>(p, u);
 #pragma unroll
             for (int n = 0; n < NP; ++n) pf[rb][n][4 * tb + e] = u[n];
           }
-      }
-      // values: byte jj of a piece is elements 2jj, 2jj+1 of it; eight tokens, regrouped by element
+    };
+    auto values = [&](const Tile& x, const v8bf(&pf)[RB][NP], int half) {
+      // byte jj of a piece is elements 2jj, 2jj+1 of it; eight tokens, regrouped by element
       float sv[2][4];
 #pragma unroll
       for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sv[tb][i] = kv4_scale((vs[tb] >> (8 * i)) & 255);
+        for (int i = 0; i < 4; ++i) sv[tb][i] = kv4_scale_of(x.vs[2 * half + tb], i);
 #pragma unroll
       for (int jj = 0; jj < VJ / 2; ++jj) {
         uint32_t u[8];
@@ -287,7 +321,7 @@ __global__ __launch_bounds__(NW * 64) void hx_kv4_attention_kernel(KaArgs a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int byte = i * PB + jj;
-            u[4 * tb + i] = ka_pair(x.v[tb][byte / 4], sv[tb][i], byte % 4);
+            u[4 * tb + i] = ka_pair(x.v[2 * half + tb][byte / 4], sv[tb][i], byte % 4);
           }
         v4i even, odd;
 #pragma unroll
@@ -303,39 +337,65 @@ __global__ __launch_bounds__(NW * 64) void hx_kv4_attention_kernel(KaArgs a) {
             o[rb][2 * jj + 1] = Mfma16<true>::run16(__builtin_bit_cast(v8bf, odd), pf[rb][n], o[rb][2 * jj + 1]);
           }
       }
-      if (__builtin_amdgcn_ballot_w64(nan_at != 0) != 0) {
+    };
+    auto put_nan = [&](const Tile& x, int t) {
+      if (__builtin_amdgcn_ballot_w64(x.nan_at != 0) != 0) {
         // rows of the count: pieces; a piece lies in one block, so all of it is NaN for the queries that see the token
-        v8bf bad;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) bad[e] = (nan_at >> e) & 1 ? (__bf16)1.f : (__bf16)0.f;
+        for (int half = 0; half < TB / 2; ++half) {
+          v8bf bad;
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          v8bf sees;
+          for (int e = 0; e < 8; ++e) bad[e] = (x.nan_at >> (8 * half + e)) & 1 ? (__bf16)1.f : (__bf16)0.f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sees[e] = 32 * t + 16 * (e >> 2) + 4 * g + (e & 3) <= last[rb] ? (__bf16)1.f : (__bf16)0.f;
-          const v4f count = Mfma16<true>::run16(bad, sees, (v4f){0.f, 0.f, 0.f, 0.f});
+          for (int rb = 0; rb < RB; ++rb) {
+            v8bf sees;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 8; ++e)
+              sees[e] = TK * t + 16 * (2 * half + (e >> 2)) + 4 * g + (e & 3) <= last[rb] ? (__bf16)1.f : (__bf16)0.f;
+            const v4f count = Mfma16<true>::run16(bad, sees, (v4f){0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-            for (int j = 0; j < VJ; ++j)
-              if (count[e] > 0.f) o[rb][j][e] = __builtin_nanf("");
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int j = 0; j < VJ; ++j)
+                if (count[e] > 0.f) o[rb][j][e] = __builtin_nanf("");
+          }
         }
       }
     };
 
     if (t_begin + w < t_end) {
+      // The loads run one tile ahead, the pages of the next one already known; past the last tile that one again, so that
+      // every step issues the same loads and the waits are for the older tile alone.
       const int t_last = t_end - 1;
-      Tile cur, next;
-      int t = t_begin + w;
-      load(cur, t, page_of(t, 0), page_of(t, 1));
-      int t1 = min(t + NW, t_last);
-      int pg0 = page_of(t1, 0), pg1 = page_of(t1, 1);
-      for (; t < t_end; t += NW) {
-        load(next, t1, pg0, pg1);
+      Tile ring[2];
+      int t = t_begin + w, t1 = min(t + NW, t_last), pages[TB];
+#pragma unroll
+      for (int tb = 0; tb < TB; ++tb) pages[tb] = page_of(t, tb);
+      load(ring[0], t, pages);
+#pragma unroll
+      for (int tb = 0; tb < TB; ++tb) pages[tb] = page_of(t1, tb);
+      auto step = [&](Tile& cur, Tile& next) {
+        load(next, t1, pages);
         t1 = min(t + 2 * NW, t_last);
-        pg0 = page_of(t1, 0), pg1 = page_of(t1, 1);
-        multiply(cur, t);
-        cur = next;
+#pragma unroll
+        for (int tb = 0; tb < TB; ++tb) pages[tb] = page_of(t1, tb);
+        scores(cur, s);
+        mask(cur, s, t);
+        vote();
+#pragma unroll
+        for (int half = 0; half < TB / 2; ++half) {
+          v8bf pf[RB][NP];
+          weights(pf, half);
+          values(cur, pf, half);
+        }
+        put_nan(cur, t);
+        t += NW;
+      };
+      for (;;) {
+        step(ring[0], ring[1]);
+        if (t >= t_end) break;
+        step(ring[1], ring[0]);
+        if (t >= t_end) break;
       }
     }
 
@@ -353,7 +413,7 @@ __global__ __launch_bounds__(NW * 64) void hx_kv4_attention_kernel(KaArgs a) {
       __syncthreads();
       for (int at = tid; at < 16 * (D / 4); at += NW * 64) {
         const int c = at / (D / 4), d = at % (D / 4) * 4;
-        const long row = row0 + 16 * rb + c;
+        const int row = row0 + 16 * rb + c;
         if (row < rows) {
           float top = stat_m[0][c];
 #pragma unroll
@@ -366,7 +426,7 @@ __global__ __launch_bounds__(NW * 64) void hx_kv4_attention_kernel(KaArgs a) {
             sum += stat_l[v][c] * f;
             acc += *(const v4f*)&joint[v][c][d] * f;
           }
-          const int i = (int)(row / G), hq = h * G + (int)(row - (long)i * G);
+          const int i = (unsigned)row / (unsigned)G, hq = h * G + row - i * G;
           const long to = (long)(start + i) * a.heads + hq;
           if (a.splits == 1) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees no key gives zeros
@@ -386,33 +446,53 @@ __global__ __launch_bounds__(NW * 64) void hx_kv4_attention_kernel(KaArgs a) {
   }
 }
 
-// Joins the splits of a row: one wave per row.
+// Joins the splits of a row: four waves per row take every fourth split, four at a time; lane i of a wave holds the
+// statistics of split i.
+#define KA_MOST 64  // splits of a row at most
 template <int D, int DT>
 __global__ __launch_bounds__(256) void hx_kv4_attention_join(KaArgs a) {
   typedef typename KaT<DT>::T T;
   constexpr int E = D / 64;
-  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (row >= (long)a.tokens * a.heads) return;
-  const int t = (int)(row / a.heads);
+  __shared__ float part[4][D];
+  const int row = blockIdx.x;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int t = (unsigned)row / (unsigned)a.heads;
   if (a.query_start && (t < a.query_start[0] || t >= a.query_start[a.batch])) return;  // behind the last sequence
-  const float* ml = a.part_ml + row * a.splits * 2;
-  float top = KA_M0;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[2 * s]);
-  float sum = 0.f, acc[E];
+  const float* ml = a.part_ml + (long)row * a.splits * 2;
+  const bool there = lane < a.splits;
+  float l = there ? ml[2 * lane + 1] : 0.f;
+  const float m = there ? ml[2 * lane] : KA_M0;
+  float top = m;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+  const float f = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - top);  // (a split without keys has written nothing else)
+  float sum = l * f;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
+  float acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float l = ml[2 * s + 1], f = __builtin_amdgcn_exp2f(ml[2 * s] - top);
-    if (l == 0.f) continue;  // a split without keys
-    sum += l * f;
-    const float* o = a.part_o + (row * a.splits + s) * D + lane * E;
+  const float* o = a.part_o + (long)row * a.splits * D + lane * E;
+  for (int s0 = w; s0 < a.splits; s0 += 16) {
+    float v[4][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += o[e] * f;
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[i][e] = o[(long)min(s0 + 4 * i, a.splits - 1) * D + e];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = s0 + 4 * i;
+      const float fs = __shfl(f, s & 63);
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (s < a.splits && fs != 0.f) acc[e] += v[i][e] * fs;
+    }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-  for (int e = 0; e < E; ++e) ((T*)a.out)[row * D + lane * E + e] = (T)(acc[e] * inv);
+  for (int e = 0; e < E; ++e) part[w][lane * E + e] = acc[e];
+  __syncthreads();
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  for (int d = threadIdx.x; d < D; d += 256) ((T*)a.out)[(long)row * D + d] = (T)((part[0][d] + part[1][d] + part[2][d] + part[3][d]) * inv);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
@@ -423,18 +503,23 @@ struct KaPlan {
 static KaPlan ka_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t max_query, int64_t max_keys, int dt) {
   KaPlan p;
   const int64_t rows = max_query * (heads / kv_heads);
-  // Four blocks of rows share a conversion of the keys and values; a head dim of 256 or an fp32 query leaves no registers for it.
-  p.rb = rows > 16 && D <= 128 && dt != HX_F32 ? 4 : 1;
-  p.nw = p.rb == 1 ? 8 : 4;
+  // Two blocks of rows share a conversion of the keys and values; a head dim of 256 or an fp32 query leaves no registers for it.
+  p.rb = rows > 16 && D <= 128 && dt != HX_F32 ? 2 : 1;
+  p.nw = 4;
   int64_t blocks = (rows + 16 * p.rb - 1) / (16 * p.rb);
   if (blocks < 1) blocks = 1;
   if (blocks > 65536) blocks = 65536;
   while (blocks > 1 && batch * kv_heads * blocks > (1l << 30)) blocks /= 2;
   p.blocks = (int)blocks;
-  // Keys are split when the rows give fewer than two workgroups per compute unit, into pieces of at least 512 keys.
-  const int64_t base = batch * kv_heads * blocks, want = (2l * hx_cu_count() + base - 1) / base, most = max_keys / 512;
+  // Keys are split, into pieces of at least 1024, until there are sixteen workgroups per compute unit (sequences differ in
+  // length, and what ends last counts) or two of the larger ones; a sequence shorter than the table's width uses fewer.
+  // Where there are four per unit without a split the joining costs more than it gives (64 sequences x 32 heads of up to
+  // 2048 keys: 42 us whole, 48 in two pieces).  One sequence of 32768 keys, 8 heads: pieces of 2048 18.4 us, 1024 14.0,
+  // 512 15.2; 32 sequences up to 32768: 122, 124, 125; 4 new tokens of 16 sequences of 8192: two per unit 40, four 47.
+  const int64_t base = batch * kv_heads * blocks, cus = hx_cu_count(), most = max_keys / KA_PIECE;
+  const int64_t want = base >= 4 * cus ? 1 : ((p.rb == 1 ? 16 : 2) * cus + base - 1) / base;
   int64_t s = want < most ? want : most;
-  p.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+  p.splits = (int)(s < 1 ? 1 : s > KA_MOST ? KA_MOST : s);
   return p;
 }
 
@@ -452,7 +537,7 @@ static int ka_check_sizes(const char* who, int64_t tokens, int64_t batch, int64_
     hx_set_error("%s: dtype must be HX_F16, HX_BF16 or HX_F32, got %d", who, dt);
     return HX_ERR_BAD_ARG;
   }
-  if (tokens > (1l << 30) || batch > (1l << 24) || width * page >= (1l << 31) - 64 || batch * kv_heads > (1l << 30)) {
+  if (tokens * heads >= (1l << 31) - 4096 || tokens > (1l << 30) || heads > 65535 || batch > (1l << 24) || width * page >= (1l << 31) - 64 || batch * kv_heads > (1l << 30)) {
     hx_set_error("%s: too many tokens, sequences or keys", who);
     return HX_ERR_UNSUPPORTED;
   }
@@ -471,11 +556,11 @@ static void ka_launch(const KaArgs& a, const KaPlan& p, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.kv_heads * a.batch * p.splits * p.blocks)), block(p.nw * 64);
   constexpr int NQ = DT == HX_BF16 ? 1 : DT == HX_F16 ? 2 : 3, NP = DT == HX_F32 ? 3 : 2;
   if (p.rb == 1) {
-    hx_launch(hx_kv4_attention_kernel<D, DT, NQ, NP, 1, 8>, grid, block, 0, s, a);
+    hx_launch(hx_kv4_attention_kernel<D, DT, NQ, NP, 1, 4, 2>, grid, block, 0, s, a);
   } else if constexpr (D <= 128 && DT != HX_F32) {
-    hx_launch(hx_kv4_attention_kernel<D, DT, NQ, NP, 4, 4>, grid, block, 0, s, a);
+    hx_launch(hx_kv4_attention_kernel<D, DT, NQ, DT == HX_BF16 ? 1 : NP, 2, 4, 2>, grid, block, 0, s, a);
   }
-  if (p.splits > 1) hx_launch(hx_kv4_attention_join<D, DT>, dim3((unsigned)(((long)a.tokens * a.heads + 3) / 4)), dim3(256), 0, s, a);
+  if (p.splits > 1) hx_launch(hx_kv4_attention_join<D, DT>, dim3((unsigned)((long)a.tokens * a.heads)), dim3(256), 0, s, a);
 }
 
 extern "C" int hx_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_codes, const void* k_scales,
@@ -516,7 +601,8 @@ extern "C" int hx_kv4_attention(const void* q, int64_t q_token_stride, int64_t q
   a.kc = (const uint8_t*)k_codes, a.ks = (const uint8_t*)k_scales, a.vc = (const uint8_t*)v_codes, a.vs = (const uint8_t*)v_scales;
   a.table = block_table, a.table_stride = table_stride, a.seq_lens = seq_lens, a.query_start = query_start;
   a.part_o = (float*)workspace, a.part_ml = need ? a.part_o + (size_t)tokens * heads * p.splits * D : nullptr;
-  a.c = scale * 1.44269504f;
+  a.negate = scale < 0.f;
+  a.c = fmaxf(fabsf(scale) * 1.44269504f, 1e-37f);  // (zero times a masked score would be NaN)
   a.tokens = (int)tokens, a.batch = (int)batch, a.heads = (int)heads, a.kv_heads = (int)kv_heads, a.pages = (int)pages;
   a.page_shift = __builtin_ctzll((unsigned long long)page), a.table_width = pages > 0 ? (int)table_width : 0, a.causal = causal != 0;
   a.splits = p.splits, a.blocks = p.blocks;

@@ -92,8 +92,12 @@ def check_attention(out, q, cache, table, lens, start, scale=None, causal=True, 
     assert (err <= most).all(), f"off by up to {float((err / most).max()):.2f} of the bound"
 
 
-def p_terms(dtype):
-    return 3 if dtype == F32 else 2
+def p_terms(dtype, dim, news, group):
+    """bf16 terms a weight is multiplied as: three for fp32; two, except where a bf16 result is rounded as coarsely itself and
+    rows are many (more than 16 for a sequence, head dims up to 128): one"""
+    if dtype == F32:
+        return 3
+    return 1 if dtype == BF and dim <= 128 and (max(news) if news else 1) * group > 16 else 2
 
 
 # (dtype, dim, page, kv_heads, group, lens, new tokens or None)

@@ -24,6 +24,7 @@ typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 
 #define HX_LDS(p) (p)
 #define HX_GLB(p) (p)
+#define HX_CONSTANT(T, p) ((const T*)(p))
 
 // global->LDS DMA: lane `l` of the wave writes `bytes` at lds_wave_base + l * bytes
 inline void hx_g2l16(const void* gptr, void* lds_wave_base) {

@@ -175,6 +175,17 @@ inline T shfl_xor(T v, int mask, int site) {
   memcpy(&v, &u, 4);
   return v;
 }
+// value of lane `src`: every lane of the wave must be active
+template <typename T>
+inline T shfl(T v, int src, int site) {
+  const int lane = (int)(thread_idx().x & 63);
+  T r = v;
+  for (int m = 1; m < 64; ++m) {  // (from the exchange that is modelled)
+    const T o = shfl_xor(v, m, site);
+    if ((lane ^ m) == src) r = o;
+  }
+  return r;
+}
 }  // namespace hxsim
 
 // ---- the gfx950 builtins the kernels use ------------------------------------------------------------------------------
@@ -192,6 +203,7 @@ inline T shfl_xor(T v, int mask, int site) {
 #define __builtin_amdgcn_mov_dpp(v, ctrl, rm, bm, bc) hxsim::mov_dpp((v), (ctrl), (rm), (bm), (bc), __LINE__)
 #define __builtin_amdgcn_permlane32_swap(a, b, fi, bc) hxsim::permlane32_swap((a), (b), __LINE__)
 #define __shfl_xor(v, mask) hxsim::shfl_xor((v), (mask), __LINE__)
+#define __shfl(v, src) hxsim::shfl((v), (src), __LINE__)
 #define __builtin_amdgcn_exp2f(x) exp2f(x)
 #define __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, cbsz, blgp, o0, s0, o1, s1) \
   hxsim::mfma_t<hxsim::MFMA_F8_32x32x64, hxs_v8i, hxs_v16f>((a), (b), (c), __LINE__)

@@ -253,7 +253,7 @@ def test_kv4_attention(dtype, dim, page, kv_heads, group, lens, news):
     cd = hx.Kv4Cache(*_dev(*cache))
     mq = max(news) if news else 1
     out = hx.kv4_attention(qd, cd, td, nd, query_start=sd, max_query_len=mq)
-    lb.check_attention(out, qd, cd, td, nd, sd, p_terms=lb.p_terms(dtype))
+    lb.check_attention(out, qd, cd, td, nd, sd, p_terms=lb.p_terms(dtype, dim, news, group))
     again = hx.kv4_attention(qd, cd, td, nd, query_start=sd, max_query_len=mq)
     assert torch.equal(out, again)
 

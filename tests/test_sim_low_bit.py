@@ -168,7 +168,7 @@ def test_kv4_write_the_last_token_of_a_slot_stays(tokens):
 def test_kv4_attention(dtype, dim, page, kv_heads, group, lens, news):
     q, cache, table, n, start = lb.attention_case(dtype, dim, page, kv_heads, group, lens, news)
     out = simops.kv4_attention(q, cache, table, n, start)
-    lb.check_attention(out, q, cache, table, n, start, p_terms=lb.p_terms(dtype))
+    lb.check_attention(out, q, cache, table, n, start, p_terms=lb.p_terms(dtype, dim, news, group))
 
 
 @pytest.mark.parametrize("dtype,news", [(BF, None), (HF, [2, 40])])
