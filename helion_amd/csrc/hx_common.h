@@ -104,6 +104,19 @@ __device__ __forceinline__ void hx_mfma_16x16x128_e4m3_acc(v4f& acc, v8i a, v8i 
   asm volatile("v_mfma_f32_16x16x128_f8f6f4 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
 
+// D(16x16 i32) += A(16 x 64 i8) * B(64 x 16 i8), in place: lane l supplies 16 bytes of row/col l%16, k = 16*(l/16) .. +15;
+// results as in the 16x16 shapes above.  hx_mfma_settle: a wait for the longest
+// of the matrix pipe's latencies, between an instruction that writes accumulators and one that reads them.
+__device__ __forceinline__ void hx_mfma_16x16x64_i8_acc(v4i& acc, v4i a, v4i b) {
+  asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void hx_acc_pin(v4i& acc) { asm volatile("" : "+a"(acc)); }  // its value is in place from here on
+__device__ __forceinline__ void hx_mfma_settle() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 __device__ __forceinline__ float hx_acc_read(float e) {
   float t;
   asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(t) : "a"(e));

@@ -24,8 +24,6 @@ struct I8Args {
   uint32_t b_max;  // last byte offset of B^T a 16-byte read may start at
 };
 
-__device__ __forceinline__ v4i i8_mfma(v4i a, v4i b, v4i c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
-
 __device__ __forceinline__ float i8_bias(const void* bias, int dt, long n) {
   return dt == HX_F32 ? ((const float*)bias)[n] : dt == HX_BF16 ? (float)((const __bf16*)bias)[n] : (float)((const _Float16*)bias)[n];
 }
@@ -102,25 +100,28 @@ __global__ __launch_bounds__(256) void hx_int8_gemm_tile(I8Args p) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < WMB; ++j) acc[i][j] = (v4i){0, 0, 0, 0};
+    for (int j = 0; j < WMB; ++j) {
+      acc[i][j] = (v4i){0, 0, 0, 0};
+      hx_acc_pin(acc[i][j]);
+    }
 
+  constexpr int EVERY = 8 * WMB >= 4 * IPW ? 4 : 2;
   // One k-tile: its MFMAs row block by row block; a fragment takes the next tile's rows as soon as its last MFMA is out,
-  // one DMA instruction follows every MFMA pair.
+  // one DMA instruction follows every EVERY MFMAs.
   auto step = [&](int kt) {
     __builtin_amdgcn_s_waitcnt(hx_vmcnt_imm((NS - 2) * IPW));  // this wave's part of tile kt+1 has landed
     __syncthreads();  // ... everybody's has, and every wave has read tile kt out of its stage
 #pragma unroll
-    for (int i = 0; i < 4 * WMB; ++i) {
-      const int bj = i & 3, bi = i >> 2;
-      acc[bj][bi] = i8_mfma(fb[bj][0], fa[bi][0], acc[bj][bi]);
-      acc[bj][bi] = i8_mfma(fb[bj][1], fa[bi][1], acc[bj][bi]);
-      if (i < IPW) issue_one(kt + NS, i);
-      if (bj == 3) load_a(bi, kt + 1);
-      if (bi == WMB - 1) load_b(bj, kt + 1);
+    for (int i = 0; i < 8 * WMB; ++i) {  // row block, half of the k-tile, column block: an accumulator rests for three others
+      const int bj = i & 3, hi = (i >> 2) & 1, bi = i >> 3;
+      hx_mfma_16x16x64_i8_acc(acc[bj][bi], fb[bj][hi], fa[bi][hi]);
+      if (i % EVERY == EVERY - 1 && i / EVERY < IPW) issue_one(kt + NS, i / EVERY);
+      if (hi && bj == 3) load_a(bi, kt + 1);
+      if (hi && bi == WMB - 1) load_b(bj, kt + 1);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  static_assert(4 * WMB >= IPW, "every DMA instruction of a k-tile has an MFMA to follow");
+  static_assert(8 * WMB >= EVERY * IPW, "every DMA instruction of a k-tile has an MFMA to follow");
   for (int t = 0; t < NS; ++t)
 #pragma unroll
     for (int i = 0; i < IPW; ++i) issue_one(t, i);
@@ -130,8 +131,10 @@ __global__ __launch_bounds__(256) void hx_int8_gemm_tile(I8Args p) {
   for (int f = 0; f < WMB; ++f) load_a(f, 0);
 #pragma unroll
   for (int f = 0; f < 4; ++f) load_b(f, 0);
+  hx_mfma_settle();
   for (int kt = 0; kt < nk; ++kt) step(kt);
   HX_WAIT_VM0();  // no DMA may still be writing this workgroup's LDS when it ends
+  hx_mfma_settle();
 
   if (SPLIT) {
     int* C = (int*)p.c + (long)blockIdx.y * p.M * p.N;
@@ -187,6 +190,170 @@ __global__ __launch_bounds__(256) void hx_int8_gemm_tile(I8Args p) {
           if (n + r <= nlast) dst[r] = o[r];
       }
     }
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// tile256: 256 x 256 outputs per workgroup, 4 waves (2 x 2) of 128 x 128: 256 accumulators and one set of 8 + 8 fragments
+// per lane, two stages of 64 KB.  The k-tile's 128 MFMAs run in two halves (columns 0..3, then 4..7 of the wave's eight
+// blocks): under the first one the DMA of tile kt+2 goes out into this tile's own stage, whose fragments are all in
+// registers; between the halves "tile kt+1 has landed" is awaited; under the second the fragments of tile kt+1 replace
+// those that have had their last MFMA.  Rows past M or N re-read the last one and are not stored.
+// ------------------------------------------------------------------------------------------
+template <int OUT, bool KT>
+__global__ __launch_bounds__(256) void hx_int8_gemm_tile256(I8Args p) {
+  typedef typename OutT<OUT>::T out_t;
+  constexpr int TILE = 256 * I8_BK;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2][2][TILE];  // [stage][A|B]
+
+  int tm, tn;
+  {  // every XCD (workgroup i runs on XCD i % 8) walks a contiguous range of a raster eight tile rows tall
+    const int nwg = gridDim.x, wg = blockIdx.x, per = nwg >> 3, rem = nwg & 7, xcd = wg & 7, loc = wg >> 3;
+    const int tile = xcd < rem ? xcd * (per + 1) + loc : rem * (per + 1) + (xcd - rem) * per + loc;
+    const int group = 8 * (nwg / p.tiles_m), first = (tile / group) * 8, gm = min(p.tiles_m - first, 8);
+    tm = first + (tile % group) % gm;
+    tn = (tile % group) / gm;
+  }
+  const long m0 = (long)tm * 256, n0 = (long)tn * 256;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = w >> 1, wn = w & 1;
+
+  // ---- DMA: wave w fetches rows 64w .. 64w+63 of both tiles, eight rows per instruction
+  const int lrow = lane >> 3, lpos = lane & 7;
+  uint32_t a_vo[8], b_vo[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t chunk = (uint32_t)((lpos ^ ((4 * (i & 1) + (lrow >> 1)) & 7)) * 16);
+    a_vo[i] = (uint32_t)min((int)m0 + 64 * w + 8 * i + lrow, p.M - 1) * (uint32_t)p.lda + chunk;
+    b_vo[i] = (uint32_t)min((int)n0 + 64 * w + 8 * i + lrow, p.N - 1) * (uint32_t)p.ldb + chunk;
+  }
+  const uint8_t *A = p.a, *B = p.b;
+  const uint32_t b_max = p.b_max, lds0 = hx_lds_addr(&smem[0][0][0]) + (uint32_t)w * 64 * 128;
+  const int nk = p.nk;
+  auto issue_one = [&](int kt, int stage, int i) {
+    const uint32_t la = lds0 + (uint32_t)stage * 2 * TILE;
+    const long t = (long)kt * I8_BK;
+    if (i < 8) hx_g2l16_s(hx_uniform_ptr(A + t), a_vo[i], la + i * 1024);
+    else if (KT) hx_g2l16_s(hx_uniform_ptr(B), min(b_vo[i - 8] + (uint32_t)t, b_max), la + TILE + (i - 8) * 1024);
+    else hx_g2l16_s(hx_uniform_ptr(B + t), b_vo[i - 8], la + TILE + (i - 8) * 1024);
+  };
+
+  const int r16 = lane & 15, gq = lane >> 4;
+  const int kq = (gq >> 1) ^ ((gq & 1) * 3);
+  const int x16 = ((2 * kq) ^ ((r16 >> 1) & 7)) * 16;
+  const int a_base = (wm * 128 + r16) * 128, b_base = (wn * 128 + r16) * 128;
+  v4i fa[8][2], fb[8][2];
+  auto load_a = [&](int stage, int f) {
+    const uint8_t* st = &smem[stage][0][0] + a_base + f * 2048;
+    fa[f][0] = *(const v4i*)(st + x16), fa[f][1] = *(const v4i*)(st + (x16 ^ 16));
+  };
+  auto load_b = [&](int stage, int f) {
+    const uint8_t* st = &smem[stage][1][0] + b_base + f * 2048;
+    fb[f][0] = *(const v4i*)(st + x16), fb[f][1] = *(const v4i*)(st + (x16 ^ 16));
+  };
+  // acc[bj][bi][r] is C[m0 + wm*128 + 16 bi + lane%16][n0 + wn*128 + 16 bj + 4*(lane/16) + r]
+  v4i acc[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      acc[i][j] = (v4i){0, 0, 0, 0};
+      hx_acc_pin(acc[i][j]);
+    }
+
+  auto ktile = [&](int kt, auto with_dma) {
+    constexpr bool dma = decltype(with_dma)::value;
+    const int stage = kt & 1;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) {
+      const int bj = i & 3, hi = (i >> 2) & 1, bi = i >> 3;
+      hx_mfma_16x16x64_i8_acc(acc[bj][bi], fb[bj][hi], fa[bi][hi]);
+      if (dma && (i & 3) == 3) issue_one(kt + 2, stage, i >> 2);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (dma) __builtin_amdgcn_s_waitcnt(hx_vmcnt_imm(16));  // tile kt+1 has landed, tile kt+2 stays in flight
+    else HX_WAIT_VM0();
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 64; ++i) {
+      const int bj = 4 + (i & 3), hi = (i >> 2) & 1, bi = i >> 3;
+      hx_mfma_16x16x64_i8_acc(acc[bj][bi], fb[bj][hi], fa[bi][hi]);
+      if ((i & 7) == 7) load_a(stage ^ 1, bi);
+      if ((i & 15) == 2) load_b(stage ^ 1, i >> 4);
+      if (i >= 60) load_b(stage ^ 1, 4 + (i - 60));  // its last MFMA of this tile is out
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();  // every wave has read tile kt+1's fragments: its stage is free
+  };
+#pragma unroll
+  for (int i = 0; i < 16; ++i) issue_one(0, 0, i);
+  if (nk > 1) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) issue_one(1, 1, i);
+    __builtin_amdgcn_s_waitcnt(hx_vmcnt_imm(16));
+  } else {
+    HX_WAIT_VM0();
+  }
+  __syncthreads();
+#pragma unroll
+  for (int f = 0; f < 8; ++f) load_a(0, f), load_b(0, f);
+  __syncthreads();
+  hx_mfma_settle();
+  int kt = 0;
+  for (; kt + 2 < nk; ++kt) ktile(kt, std::true_type{});
+  for (; kt < nk; ++kt) ktile(kt, std::false_type{});  // the last two have nothing left to fetch
+  // (past the last tile the fragments are refilled from a stage that holds an older tile, or nothing; nobody uses them)
+  hx_mfma_settle();
+
+  // ---- epilogue: 32 rows x 128 columns at a time through the wave's own quarter of the LDS, so that every store
+  // instruction writes whole row pieces
+  constexpr int ESZ = (int)sizeof(out_t), ROWB = 128 * ESZ, RSTR = ROWB + 16, LPR = ROWB / 16, RPI = 64 / LPR;
+  typedef out_t ov4 __attribute__((ext_vector_type(4)));
+  uint8_t* st = &smem[0][0][0] + w * TILE;
+  out_t* C = (out_t*)p.c;
+  const long col0 = n0 + wn * 128;
+  v4f sb[8], add[8];
+#pragma unroll
+  for (int bj = 0; bj < 8; ++bj)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const long n = min(col0 + 16 * bj + 4 * gq + r, (long)p.N - 1);
+      sb[bj][r] = p.sb[n];
+      add[bj][r] = p.bias ? i8_bias(p.bias, p.bias_dt, n) : 0.f;
+    }
+  const bool vec = p.ldc % (16 / ESZ) == 0 && ((uintptr_t)C & 15) == 0;
+#pragma unroll
+  for (int b32 = 0; b32 < 4; ++b32) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float sa = p.sa[min(m0 + wm * 128 + b32 * 32 + h * 16 + r16, (long)p.M - 1)];
+#pragma unroll
+      for (int bj = 0; bj < 8; ++bj) {
+        ov4 o;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = (out_t)((float)acc[bj][2 * b32 + h][r] * sa * sb[bj][r] + add[bj][r]);
+        *(ov4*)(st + (h * 16 + r16) * RSTR + (bj * 16 + 4 * gq) * ESZ) = o;
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // (the LDS runs one wave's operations in order)
+#pragma unroll
+    for (int q = 0; q < 32 / RPI; ++q) {
+      const int row = q * RPI + lane / LPR;
+      const v4i v = *(const v4i*)(st + row * RSTR + lane % LPR * 16);
+      const long m = m0 + wm * 128 + b32 * 32 + row, n = col0 + lane % LPR * (16 / ESZ);
+      if (m < p.M) {
+        out_t* dst = C + m * p.ldc + n;
+        if (vec && n + 16 / ESZ <= p.N) {
+          *(v4i*)dst = v;
+        } else {
+          const out_t* e = (const out_t*)&v;
+          for (int b = 0; b < 16 / ESZ; ++b)
+            if (n + b < p.N) dst[b] = e[b];
+        }
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
 }
 
@@ -255,6 +422,15 @@ struct I8Plan {
   size_t a_off, b_off, part_off, bytes;
 };
 
+// Rows of the tile: 64 or 128 (of 128 columns), or 256 (of 256).  All run one workgroup per compute unit, so a launch takes
+// ceil(tiles / 256) rounds of nk steps plus what a tile costs outside its loop, and the cheaper estimate wins.
+static int i8_rows(int64_t M, int64_t N, int64_t nk) {
+  if (M <= 64) return 64;
+  const int64_t cus = hx_cu_count();
+  auto rounds = [&](int64_t t) { return (((M + t - 1) / t) * ((N + t - 1) / t) + cus - 1) / cus; };
+  return M > 128 && rounds(256) * (150 * nk + 600) <= rounds(128) * (45 * nk + 460) ? 256 : 128;
+}
+
 static I8Plan i8_plan(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb_k, int64_t ldb_n, bool a_aligned, bool b_aligned) {
   I8Plan p;
   p.ka = (K + I8_BK - 1) / I8_BK * I8_BK;
@@ -262,12 +438,12 @@ static I8Plan i8_plan(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb_
   p.copy_b = !(b_rows && K % 16 == 0);
   p.tail = !p.copy_b && K % I8_BK != 0;
   p.copy_a = !(K % I8_BK == 0 && lda % 16 == 0 && a_aligned && M * lda < (1LL << 32));
-  p.bm = M <= 64 ? 64 : 128;
-  p.bn = 128;
+  p.bm = i8_rows(M, N, p.ka / I8_BK);
+  p.bn = p.bm == 256 ? 256 : 128;
   const int64_t tiles = ((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn), nk = p.ka / I8_BK;
   // Few tiles and a long K: the k-tiles of a tile are divided among workgroups, eight at least for each, and the partial
   // sums stay below 32 MB.
-  int64_t s = hx_cu_count() / tiles;
+  int64_t s = p.bm == 256 ? 1 : hx_cu_count() / tiles;
   if (s > nk / 8) s = nk / 8;
   while (s > 1 && s * M * N * 4 > (32LL << 20)) --s;
   p.splits = 1, p.kt_per_split = 0;
@@ -338,7 +514,10 @@ static void i8_launch(I8Args a, const I8Plan& p, void* ws, hipStream_t s) {
   const dim3 grid((unsigned)(a.tiles_m * ((a.N + p.bn - 1) / p.bn)), (unsigned)p.splits);
   void* c = a.c;
   if (p.splits > 1) a.c = (uint8_t*)ws + p.part_off;
-  if (p.bm == 64) i8_launch_tile<OUT, 64>(a, p, grid, s);
+  if (p.bm == 256) {
+    if (p.tail) hx_launch(hx_int8_gemm_tile256<OUT, true>, grid, dim3(256), 0, s, a);
+    else hx_launch(hx_int8_gemm_tile256<OUT, false>, grid, dim3(256), 0, s, a);
+  } else if (p.bm == 64) i8_launch_tile<OUT, 64>(a, p, grid, s);
   else i8_launch_tile<OUT, 128>(a, p, grid, s);
   if (p.splits > 1) {
     const int* part = (const int*)a.c;

@@ -58,6 +58,9 @@ inline v4f hx_mfma_16x16x128_e4m3(v8i a, v8i b, v4f c) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
 }
 
+inline void hx_mfma_16x16x64_i8_acc(v4i& acc, v4i a, v4i b) { acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, acc, 0, 0, 0); }
+inline void hx_acc_pin(v4i&) {}
+inline void hx_mfma_settle() {}
 inline float hx_acc_read(float e) { return e; }
 inline void hx_mfma_16x16x128_e4m3_overwrite(v4f& acc, v8i a, v8i b) { acc = hx_mfma_16x16x128_e4m3(a, b, (v4f){0.f, 0.f, 0.f, 0.f}); }
 inline void hx_mfma_16x16x128_e4m3_acc(v4f& acc, v8i a, v8i b) { acc = hx_mfma_16x16x128_e4m3(a, b, acc); }
