@@ -46,14 +46,13 @@ __global__ __launch_bounds__(256) void hx_int8_gemm_tile(I8Args p) {
 
   const int kt0 = SPLIT ? p.kt_per_split * (int)blockIdx.y : 0;
   const int nk = SPLIT ? min(p.kt_per_split, p.nk - kt0) : p.nk;
-  // 256 consecutive tiles of a raster of eight tile rows at a time, in blocks of 32 per XCD (workgroup i runs on XCD i % 8)
+  // 256 consecutive tiles of a raster of eight tile rows at a time, in eight contiguous pieces, one per XCD (workgroup i
+  // runs on XCD i % 8), so that the tiles resident on one share panels of A and B in its L2
   int tm, tn;
   {
-    const int nwg = gridDim.x, wg = blockIdx.x, chunk = wg >> 8, tiles_n = nwg / p.tiles_m;
-    const int rem = nwg & 255, l = wg & 255;
-    const int tile = chunk < (nwg >> 8) ? (chunk << 8) + ((wg & 7) << 5) + ((wg >> 3) & 31)
-                     : (rem & 7) == 0   ? (chunk << 8) + (l & 7) * (rem >> 3) + (l >> 3)
-                                        : wg;
+    const int nwg = gridDim.x, wg = blockIdx.x, run = wg & ~255, n = min(nwg - run, 256), l = wg & 255, tiles_n = nwg / p.tiles_m;
+    const int per = n >> 3, rem = n & 7, xcd = l & 7;
+    const int tile = run + xcd * per + min(xcd, rem) + (l >> 3);
     const int group = 8 * tiles_n, first = (tile / group) * 8, gm = min(p.tiles_m - first, 8);
     tm = first + (tile % group) % gm;
     tn = (tile % group) / gm;
@@ -357,6 +356,121 @@ __global__ __launch_bounds__(256) void hx_int8_gemm_tile256(I8Args p) {
   }
 }
 
+// ------------------------------------------------------------------------------------------
+// skinny: M <= 32 (MB blocks of 16 rows).  The weights are read once, straight into registers; one workgroup of 8 waves per
+// compute unit walks groups of 16 columns, wave w multiplies the 128-byte k-steps w, w+8, ... of each and keeps the rows of
+// A for them in registers all along.  One load instruction covers eight rows of 128 bytes (whole lines): lane (j = lane%16,
+// g = lane/16) takes chunk 2g + (j&1) of row j>>1, a second instruction rows 8..15 with the other chunk; one exchange with
+// the neighbouring lane leaves chunks 2g and 2g+1 of row (j>>1) + 8 (j&1), two MFMA operands.  The registers of a step are
+// refilled with the same step of the next group as soon as the operands are built, so that about one group per wave (128 KB
+// per compute unit) is in flight, also across the barrier that adds up the eight waves' sums.
+// NS > 0: every wave has NS steps and the loads in flight can be counted; NS = 0: any number up to eight, and a K that is
+// not a multiple of 128 (B's rows are read on, clamped to the end of the matrix: A is zero there).
+// split (gridDim.y > 1): workgroup row y adds up its steps into its own slab of 32-bit integers.
+// ------------------------------------------------------------------------------------------
+#define I8S_WAVES 8
+#define I8S_STEPS 8
+template <int OUT, int NS, int MB, bool SPLIT>
+__global__ __launch_bounds__(512) void hx_int8_gemm_skinny(I8Args p) {
+  typedef typename OutT<OUT>::T out_t;
+  constexpr bool FULL = NS > 0;
+  __shared__ __attribute__((aligned(16))) int red[2][I8S_WAVES][MB * 4][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int j = lane & 15, g = lane >> 4, odd = j & 1;
+  const int first = SPLIT ? p.kt_per_split * (int)blockIdx.y : 0;                  // k-steps of this workgroup
+  const int steps = SPLIT ? min(p.kt_per_split, p.nk - first) : p.nk;
+  const int nmine = FULL ? NS : (steps - w + I8S_WAVES - 1) / I8S_WAVES;
+  const int ncg = (p.N + 15) >> 4, grid = (int)gridDim.x;
+
+  const int c_lo = (2 * g + odd) * 16, c_hi = (2 * g + (odd ^ 1)) * 16;
+  const long k0 = (long)(first + w) * I8_BK;
+  const uint8_t *p0, *p1;
+  const uint8_t* end = p.b + p.b_max;
+  auto point_at = [&](int cg) {
+    p0 = p.b + (long)min(cg * 16 + (j >> 1), p.N - 1) * p.ldb + c_lo + k0;
+    p1 = p.b + (long)min(cg * 16 + 8 + (j >> 1), p.N - 1) * p.ldb + c_hi + k0;
+  };
+  v4i x0[I8S_STEPS], x1[I8S_STEPS];
+  auto load_step = [&](int s) {
+    const uint8_t *q0 = p0 + (long)s * I8S_WAVES * I8_BK, *q1 = p1 + (long)s * I8S_WAVES * I8_BK;
+    if (!FULL) q0 = q0 < end ? q0 : end, q1 = q1 < end ? q1 : end;
+    x0[s] = __builtin_nontemporal_load((const v4i*)q0);
+    x1[s] = __builtin_nontemporal_load((const v4i*)q1);
+  };
+  int cg = (int)blockIdx.x;  // grid <= ncg: every workgroup has a group
+  point_at(cg);
+#pragma unroll
+  for (int s = 0; s < I8S_STEPS; ++s)
+    if (FULL ? s < NS : s < nmine) load_step(s);
+
+  // rows of A like those of B: lane (j, g) ends up with chunks 2g, 2g+1 of row 16 mb + (j>>1) + 8 (j&1)
+  v4i alo[MB][I8S_STEPS], ahi[MB][I8S_STEPS];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    const uint8_t* ap0 = p.a + (long)min(mb * 16 + (j >> 1), p.M - 1) * p.lda + c_lo + k0;
+    const uint8_t* ap1 = p.a + (long)min(mb * 16 + 8 + (j >> 1), p.M - 1) * p.lda + c_hi + k0;
+#pragma unroll
+    for (int s = 0; s < I8S_STEPS; ++s)
+      if (FULL ? s < NS : s < nmine) {
+        const v4i a0 = *(const v4i*)(ap0 + (long)s * I8S_WAVES * I8_BK), a1 = *(const v4i*)(ap1 + (long)s * I8S_WAVES * I8_BK);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          alo[mb][s][d] = odd ? a1[d] : a0[d];
+          ahi[mb][s][d] = __builtin_amdgcn_mov_dpp(odd ? a0[d] : a1[d], 0xB1, 0xF, 0xF, true);  // from lane ^ 1
+        }
+        if (MB > 1) __builtin_amdgcn_sched_barrier(0);  // bounds the raw lines in flight
+      }
+  }
+
+  int parity = 0;
+  // whether there is a next group is a property of the body, so that its loads stay countable
+  auto one_group = [&](auto more_c) {
+    constexpr bool more = decltype(more_c)::value;
+    if (more) point_at(cg + grid);
+    v4i acc[MB];
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) acc[mb] = (v4i){0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < I8S_STEPS; ++s)
+      if (FULL ? s < NS : s < nmine) {
+        v4i lo, hi;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          lo[d] = odd ? x1[s][d] : x0[s][d];
+          hi[d] = __builtin_amdgcn_mov_dpp(odd ? x0[s][d] : x1[s][d], 0xB1, 0xF, 0xF, true);
+        }
+        if (more) load_step(s);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+          acc[mb] = __builtin_amdgcn_mfma_i32_16x16x64_i8(alo[mb][s], lo, acc[mb], 0, 0, 0);
+          acc[mb] = __builtin_amdgcn_mfma_i32_16x16x64_i8(ahi[mb][s], hi, acc[mb], 0, 0, 0);
+        }
+      }
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) red[parity][w][4 * mb + r][lane] = acc[mb][r];
+    __syncthreads();
+    if (tid < 256 * MB) {
+      const int l2 = tid & 63, rr = tid >> 6;
+      int sum = 0;
+#pragma unroll
+      for (int ww = 0; ww < I8S_WAVES; ++ww) sum += red[parity][ww][rr][l2];
+      const int j2 = l2 & 15, i2 = 4 * (l2 >> 4) + (rr & 3);  // column and row of the MFMA
+      const int m = 16 * (rr >> 2) + (i2 >> 1) + 8 * (i2 & 1), n = cg * 16 + (j2 >> 1) + 8 * (j2 & 1);
+      if (m < p.M && n < p.N) {
+        if (SPLIT) ((int*)p.c)[((long)blockIdx.y * p.M + m) * p.N + n] = sum;
+        else ((out_t*)p.c)[(long)m * p.ldc + n] = (out_t)((float)sum * p.sa[m] * p.sb[n] + (p.bias ? i8_bias(p.bias, p.bias_dt, n) : 0.f));
+      }
+    }
+    parity ^= 1;  // the next group writes the other buffer: one barrier per group is enough
+    cg += grid;
+  };
+  while (cg + grid < ncg) one_group(std::true_type{});
+  one_group(std::false_type{});
+}
+
 // split-K: C = cast(sum over the slabs [split][M][N] * scales + bias); one thread per four columns
 template <int OUT>
 __global__ __launch_bounds__(256) void hx_int8_gemm_split_reduce(I8Args p, const int* __restrict__ part, int splits) {
@@ -419,6 +533,7 @@ struct I8Plan {
   bool copy_a, copy_b, tail;  // tail: K % 128 != 0 with B read in place
   int64_t ka;                 // padded row length of the copies
   int bm, bn, splits, kt_per_split;
+  int ns;                     // skinny kernel: steps per wave as a constant, 0 not constant; -1 another kernel
   size_t a_off, b_off, part_off, bytes;
 };
 
@@ -431,6 +546,34 @@ static int i8_rows(int64_t M, int64_t N, int64_t nk) {
   return M > 128 && rounds(256) * (150 * nk + 600) <= rounds(128) * (45 * nk + 460) ? 256 : 128;
 }
 
+static void i8_offsets(I8Plan& p, int64_t M, int64_t N) {
+  size_t at = 0;
+  auto take = [&](bool want, int64_t bytes) {
+    const size_t here = at;
+    if (want) at += ((size_t)bytes + 255) & ~(size_t)255;
+    return here;
+  };
+  p.a_off = take(p.copy_a, M * p.ka);
+  p.b_off = take(p.copy_b, N * p.ka);
+  p.part_off = take(p.splits > 1, (int64_t)p.splits * M * N * 4);
+  p.bytes = at;
+}
+
+// Up to 32 rows: k in pieces of at most 64 steps per workgroup (eight waves of up to eight), and in more of them while the
+// groups of 16 columns do not fill the compute units; at least eight steps each.
+static I8Plan i8_plan_skinny(I8Plan p, int64_t M, int64_t N, int64_t K) {
+  const int64_t nk = p.ka / I8_BK, ncg = (N + 15) / 16;
+  int64_t s = (nk + 63) / 64;
+  while (ncg * s < hx_cu_count() && nk / (2 * s) >= 8) s *= 2;
+  const int64_t per = ((nk + s - 1) / s + 7) / 8 * 8;
+  p.bm = 16, p.bn = 16;
+  p.splits = (int)((nk + per - 1) / per);
+  p.kt_per_split = p.splits > 1 ? (int)per : 0;
+  p.ns = nk % per == 0 && !p.tail ? (int)(per / 8) : 0;
+  i8_offsets(p, M, N);
+  return p;
+}
+
 static I8Plan i8_plan(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb_k, int64_t ldb_n, bool a_aligned, bool b_aligned) {
   I8Plan p;
   p.ka = (K + I8_BK - 1) / I8_BK * I8_BK;
@@ -438,6 +581,8 @@ static I8Plan i8_plan(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb_
   p.copy_b = !(b_rows && K % 16 == 0);
   p.tail = !p.copy_b && K % I8_BK != 0;
   p.copy_a = !(K % I8_BK == 0 && lda % 16 == 0 && a_aligned && M * lda < (1LL << 32));
+  p.ns = -1;
+  if (M <= 32) return i8_plan_skinny(p, M, N, K);
   p.bm = i8_rows(M, N, p.ka / I8_BK);
   p.bn = p.bm == 256 ? 256 : 128;
   const int64_t tiles = ((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn), nk = p.ka / I8_BK;
@@ -451,16 +596,7 @@ static I8Plan i8_plan(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb_
     p.kt_per_split = (int)((nk + s - 1) / s);
     p.splits = (int)((nk + p.kt_per_split - 1) / p.kt_per_split);
   }
-  size_t at = 0;
-  auto take = [&](bool want, int64_t bytes) {
-    const size_t here = at;
-    if (want) at += ((size_t)bytes + 255) & ~(size_t)255;
-    return here;
-  };
-  p.a_off = take(p.copy_a, M * p.ka);
-  p.b_off = take(p.copy_b, N * p.ka);
-  p.part_off = take(p.splits > 1, (int64_t)p.splits * M * N * 4);
-  p.bytes = at;
+  i8_offsets(p, M, N);
   return p;
 }
 
@@ -508,13 +644,34 @@ static void i8_launch_tile(const I8Args& a, const I8Plan& p, dim3 grid, hipStrea
   }
 }
 
+template <int OUT, int MB, bool SPLIT>
+static void i8_launch_skinny(const I8Args& a, int ns, dim3 grid, hipStream_t s) {
+  switch (ns) {
+#define I8S_CASE(NS) \
+  case NS: hx_launch(hx_int8_gemm_skinny<OUT, NS, MB, SPLIT>, grid, dim3(512), 0, s, a); break;
+    I8S_CASE(1) I8S_CASE(2) I8S_CASE(3) I8S_CASE(4) I8S_CASE(5) I8S_CASE(6) I8S_CASE(7) I8S_CASE(8)
+#undef I8S_CASE
+    default: hx_launch(hx_int8_gemm_skinny<OUT, 0, MB, SPLIT>, grid, dim3(512), 0, s, a);
+  }
+}
+
 template <int OUT>
 static void i8_launch(I8Args a, const I8Plan& p, void* ws, hipStream_t s) {
   a.tiles_m = (a.M + p.bm - 1) / p.bm, a.bn = p.bn, a.kt_per_split = p.kt_per_split;
   const dim3 grid((unsigned)(a.tiles_m * ((a.N + p.bn - 1) / p.bn)), (unsigned)p.splits);
   void* c = a.c;
   if (p.splits > 1) a.c = (uint8_t*)ws + p.part_off;
-  if (p.bm == 256) {
+  if (p.ns >= 0) {
+    const int ncg = (a.N + 15) / 16, cus = hx_cu_count();
+    const dim3 sg((unsigned)(ncg < cus ? ncg : cus), (unsigned)p.splits);
+    if (p.splits > 1) {
+      if (a.M <= 16) i8_launch_skinny<HX_F32, 1, true>(a, p.ns, sg, s);
+      else i8_launch_skinny<HX_F32, 2, true>(a, p.ns, sg, s);
+    } else {
+      if (a.M <= 16) i8_launch_skinny<OUT, 1, false>(a, p.ns, sg, s);
+      else i8_launch_skinny<OUT, 2, false>(a, p.ns, sg, s);
+    }
+  } else if (p.bm == 256) {
     if (p.tail) hx_launch(hx_int8_gemm_tile256<OUT, true>, grid, dim3(256), 0, s, a);
     else hx_launch(hx_int8_gemm_tile256<OUT, false>, grid, dim3(256), 0, s, a);
   } else if (p.bm == 64) i8_launch_tile<OUT, 64>(a, p, grid, s);
