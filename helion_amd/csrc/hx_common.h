@@ -178,6 +178,16 @@ __device__ __forceinline__ float hx_e4m3_to_f32(uint8_t code) {
   return __builtin_amdgcn_cvt_f32_fp8((int)code, 0);
 }
 
+// this wave's place on its SIMD (WAVE_ID of the hardware id register)
+__device__ __forceinline__ int hx_wave_slot() { return (int)__builtin_amdgcn_s_getreg(4 | (3 << 11)); }
+
+// the largest of three in one instruction (of a NaN and a number the number; the compiler's own maxima first quiet their operands)
+__device__ __forceinline__ float hx_max3(float a, float b, float c) {
+  float d;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
+}
+
 void hx_set_error(const char* fmt, ...);
 int hx_cu_count();
 bool hx_feature(unsigned bit);  // is this opt-in kernel path (HX_FEATURE_* of the C header) switched on  // compute units of the current device (looked up once per device, 256 if the query fails)

@@ -90,8 +90,65 @@ __device__ __forceinline__ void ka_terms(float f, __bf16 (&t)[N]) {
   }
 }
 
+// One sequence and key/value head of a launch
+struct KaSeq {
+  int b, h, split, block0;
+  int G, start, n_new, rows, kv_len;
+  const int* table;
+};
+__device__ __forceinline__ bool ka_sequence(const KaArgs& a, KaSeq& q) {  // false: nothing to do
+  int id = blockIdx.x;
+  q.h = id % a.kv_heads;  // eight heads: one per XCD, whose L2 then holds that head's keys
+  id /= a.kv_heads;
+  q.b = id % a.batch;
+  id /= a.batch;
+  q.split = id % a.splits;
+  q.block0 = id / a.splits;
+  q.G = a.heads / a.kv_heads;
+  q.start = a.query_start ? ka_scalar(a.query_start + q.b) : q.b;
+  if (q.start < 0 || q.start >= a.tokens) return false;
+  q.n_new = min(a.query_start ? ka_scalar(a.query_start + q.b + 1) - q.start : 1, a.tokens - q.start);
+  q.rows = q.n_new * q.G;  // (tokens * heads < 2^31, checked by the host)
+  q.kv_len = (int)min((long)max(ka_scalar(a.seq_lens + q.b), 0), (long)a.table_width << a.page_shift);
+  q.table = a.table + q.b * a.table_stride;
+  return true;
+}
+
+// The queries of RB blocks of 16 rows from row0 on as second operands: column c = lane % 16 of block rb is row
+// row0 + 16 rb + c (past the last row: that one again).  last: the last key each of them sees.
+template <int D, int DT, int NQ, int RB>
+__device__ __forceinline__ void ka_queries(const KaArgs& a, const KaSeq& q, int row0, v8bf (&qf)[RB][NQ][D / 32], int (&last)[RB]) {
+  typedef typename KaT<DT>::T T;
+  typedef T Tv __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  const int r16 = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const int row = min(row0 + 16 * rb + r16, q.rows - 1);
+    const int i = (unsigned)row / (unsigned)q.G, hq = q.h * q.G + row - i * q.G;
+    last[rb] = a.causal ? q.kv_len - q.n_new + i : q.kv_len - 1;
+    const T* qp = (const T*)a.q + (q.start + i) * a.q_token_stride + hq * a.q_head_stride + D / 4 * g;
+#pragma unroll
+    for (int m = 0; m < D / 32; ++m) {
+      const Tv raw = *(const Tv*)(qp + 8 * m);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        __bf16 t[NQ];
+        ka_terms<NQ>(a.negate ? -(float)raw[e] : (float)raw[e], t);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) qf[rb][n][m][e] = t[n];
+      }
+    }
+  }
+}
+
+// Rows in blocks of 16 RB; the waves of the workgroup take key tiles in turn and join what they have at the end.
+template <int D, int NW>
+struct KaFewLds {
+  float joint[NW][16][D + 4];  // (padded rows)
+  float stat_m[NW][16], stat_l[NW][16];
+};
 template <int D, int DT, int NQ, int NP, int RB, int NW, int TB>
-__global__ __launch_bounds__(NW * 64, RB > 1 || D > 128 || DT == HX_F32 ? 2 : D == 64 ? 4 : DT == HX_BF16 ? 3 : 2) void hx_kv4_attention_kernel(KaArgs a) {
+__device__ __forceinline__ void ka_few(const KaArgs& a, const KaSeq& q, KaFewLds<D, NW>& lds) {
   typedef typename KaT<DT>::T T;
   constexpr bool NT = RB == 1;
   constexpr int DG = D / 4;    // elements of a key per lane
@@ -99,29 +156,14 @@ __global__ __launch_bounds__(NW * 64, RB > 1 || D > 128 || DT == HX_F32 ? 2 : D 
   constexpr int PB = D / 32;   // bytes of a piece = scales of a token = dwords of values per lane and 16 keys
   constexpr int VJ = D / 16;   // MFMAs of the second product
   constexpr int TK = 16 * TB;  // keys of a tile
-  constexpr int OSTR = D + 4;  // row stride of the joining buffer, in floats
-  __shared__ __attribute__((aligned(16))) float joint[NW][16][OSTR];
-  __shared__ float stat_m[NW][16], stat_l[NW][16];
-
-  int id = blockIdx.x;
-  const int h = id % a.kv_heads;  // eight heads: one per XCD, whose L2 then holds that head's keys
-  id /= a.kv_heads;
-  const int b = id % a.batch;
-  id /= a.batch;
-  const int split = id % a.splits;
-  const int block0 = id / a.splits;
-
+  auto& joint = lds.joint;
+  auto& stat_m = lds.stat_m;
+  auto& stat_l = lds.stat_l;
+  const int h = q.h, split = q.split, block0 = q.block0, G = q.G, start = q.start, n_new = q.n_new, rows = q.rows, kv_len = q.kv_len;
+  const int* table = q.table;
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int G = a.heads / a.kv_heads;
-  const int start = a.query_start ? ka_scalar(a.query_start + b) : b;
-  int n_new = a.query_start ? ka_scalar(a.query_start + b + 1) - start : 1;
-  if (start < 0 || start >= a.tokens) return;
-  n_new = min(n_new, a.tokens - start);
   const int pm = (1 << a.page_shift) - 1;
-  const int kv_len = (int)min((long)max(ka_scalar(a.seq_lens + b), 0), (long)a.table_width << a.page_shift);
-  const int* table = a.table + b * a.table_stride;
-  const int rows = n_new * G;  // (tokens * heads < 2^31, checked by the host)
 
   // where this lane's share of 16 keys lies
   const uint32_t kc_off = r16 * (D / 2) + g * (DG / 2), vc_off = (g * 16 + r16) * (4 * PB);
@@ -135,28 +177,9 @@ __global__ __launch_bounds__(NW * 64, RB > 1 || D > 128 || DT == HX_F32 ? 2 : D 
     const int piece = max((tiles + a.splits - 1) / a.splits, a.splits > 1 ? KA_PIECE / TK : 1);
     const int t_begin = min(split * piece, tiles), t_end = min(t_begin + piece, tiles);
 
-    // ---- this wave's queries: column c = lane % 16 of block rb is row row0 + 16 rb + c
     v8bf qf[RB][NQ][KM];
-    int last[RB];  // the last key the row sees
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const int row = min(row0 + 16 * rb + r16, rows - 1);
-      const int i = (unsigned)row / (unsigned)G, hq = h * G + row - i * G;
-      last[rb] = a.causal ? kv_len - n_new + i : kv_len - 1;
-      const T* qp = (const T*)a.q + (start + i) * a.q_token_stride + hq * a.q_head_stride + DG * g;
-      typedef T Tv __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-#pragma unroll
-      for (int m = 0; m < KM; ++m) {
-        const Tv raw = *(const Tv*)(qp + 8 * m);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          __bf16 t[NQ];
-          ka_terms<NQ>(a.negate ? -(float)raw[e] : (float)raw[e], t);
-#pragma unroll
-          for (int n = 0; n < NQ; ++n) qf[rb][n][m][e] = t[n];
-        }
-      }
-    }
+    int last[RB];
+    ka_queries<D, DT, NQ, RB>(a, q, row0, qf, last);
 
     v4f o[RB][VJ];
     float mx[RB], l[RB];
@@ -446,6 +469,15 @@ __global__ __launch_bounds__(NW * 64, RB > 1 || D > 128 || DT == HX_F32 ? 2 : D 
   }
 }
 
+template <int D, int DT, int NQ, int NP, int RB, int NW, int TB>
+__global__ __launch_bounds__(NW * 64, RB > 1 || D > 128 || DT == HX_F32 ? 2 : D == 64 ? 4 : DT == HX_BF16 ? 3 : 2) void hx_kv4_attention_kernel(KaArgs a) {
+  __shared__ __attribute__((aligned(16))) KaFewLds<D, NW> lds;
+  KaSeq q;
+  if (ka_sequence(a, q)) ka_few<D, DT, NQ, NP, RB, NW, TB>(a, q, lds);
+}
+
+#include "kv4_attention_rows.h"
+
 // Joins the splits of a row: four waves per row take every fourth split, four at a time; lane i of a wave holds the
 // statistics of split i.
 #define KA_MOST 64  // splits of a row at most
@@ -498,6 +530,7 @@ __global__ __launch_bounds__(256) void hx_kv4_attention_join(KaArgs a) {
 // ---- host side ------------------------------------------------------------------------------------------------------
 struct KaPlan {
   int rb, nw, blocks, splits;
+  bool many;  // hx_kv4_attention_rows
 };
 
 static KaPlan ka_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t max_query, int64_t max_keys, int dt) {
@@ -506,7 +539,18 @@ static KaPlan ka_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D,
   // Two blocks of rows share a conversion of the keys and values; a head dim of 256 or an fp32 query leaves no registers for it.
   p.rb = rows > 16 && D <= 128 && dt != HX_F32 ? 2 : 1;
   p.nw = 4;
-  int64_t blocks = (rows + 16 * p.rb - 1) / (16 * p.rb);
+  p.many = false;
+  // 128 rows per workgroup with the conversion shared, or 32 with the keys divided among the waves: both run two workgroups
+  // per compute unit; for 128 keys the former takes 4.5 us in whole rounds (the workgroups end together), the latter 1.2 in
+  // as many rounds as it takes.  2048 tokens over 10240 keys 323 and 340 us, 8 x 512 over 2048 139 and 164; but 12 x 200
+  // over 4000 221 and 198, 2 x 512 over 4096 109 and 83.
+  if (p.rb == 2 && rows > 64) {
+    const int64_t slots = 2 * hx_cu_count(), pairs = batch * kv_heads;
+    const int64_t many = (pairs * ((rows + KR_ROWS - 1) / KR_ROWS) + slots - 1) / slots * slots * 45, few = pairs * ((rows + 31) / 32) * 12;
+    p.many = many < few;
+  }
+  const int64_t per = p.many ? KR_ROWS : 16 * p.rb;
+  int64_t blocks = (rows + per - 1) / per;
   if (blocks < 1) blocks = 1;
   if (blocks > 65536) blocks = 65536;
   while (blocks > 1 && batch * kv_heads * blocks > (1l << 30)) blocks /= 2;
@@ -517,7 +561,7 @@ static KaPlan ka_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D,
   // 2048 keys: 42 us whole, 48 in two pieces).  One sequence of 32768 keys, 8 heads: pieces of 2048 18.4 us, 1024 14.0,
   // 512 15.2; 32 sequences up to 32768: 122, 124, 125; 4 new tokens of 16 sequences of 8192: two per unit 40, four 47.
   const int64_t base = batch * kv_heads * blocks, cus = hx_cu_count(), most = max_keys / KA_PIECE;
-  const int64_t want = base >= 4 * cus ? 1 : ((p.rb == 1 ? 16 : 2) * cus + base - 1) / base;
+  const int64_t want = base >= 4 * cus || p.many ? 1 : ((p.rb == 1 ? 16 : 2) * cus + base - 1) / base;
   int64_t s = want < most ? want : most;
   p.splits = (int)(s < 1 ? 1 : s > KA_MOST ? KA_MOST : s);
   return p;
@@ -555,7 +599,9 @@ template <int D, int DT>
 static void ka_launch(const KaArgs& a, const KaPlan& p, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.kv_heads * a.batch * p.splits * p.blocks)), block(p.nw * 64);
   constexpr int NQ = DT == HX_BF16 ? 1 : DT == HX_F16 ? 2 : 3, NP = DT == HX_F32 ? 3 : 2;
-  if (p.rb == 1) {
+  if (p.many) {
+    if constexpr (D <= 128 && DT != HX_F32) hx_launch(hx_kv4_attention_rows<D, DT, NQ, DT == HX_BF16 ? 1 : NP>, grid, dim3(KR_WAVES * 64), 0, s, a);
+  } else if (p.rb == 1) {
     hx_launch(hx_kv4_attention_kernel<D, DT, NQ, NP, 1, 4, 2>, grid, block, 0, s, a);
   } else if constexpr (D <= 128 && DT != HX_F32) {
     hx_launch(hx_kv4_attention_kernel<D, DT, NQ, DT == HX_BF16 ? 1 : NP, 2, 4, 2>, grid, block, 0, s, a);

@@ -104,6 +104,9 @@ struct OutT<HX_F32> {
 #define HX_CVT_PK_E4M3(a, b, old, hi) __builtin_amdgcn_cvt_pk_fp8_f32((a), (b), (old), (hi))
 inline float hx_e4m3_to_f32(uint8_t code) { return __builtin_amdgcn_cvt_f32_fp8((int)code, 0); }
 
+inline int hx_wave_slot() { return (int)(threadIdx.x >> 6); }
+inline float hx_max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
 void hx_set_error(const char* fmt, ...);
 int hx_cu_count();
 bool hx_feature(unsigned bit);

@@ -245,7 +245,8 @@ def test_kv4_refusals():
 @pytest.mark.parametrize("dtype,dim,page,kv_heads,group,lens,news", lb.ATTENTION + [
     (BF, 128, 64, 8, 8, [2000, 1, 777, 0, 4096], None), (HF, 128, 16, 8, 4, [517], None), (HF, 64, 16, 32, 1, [300, 2048], None),
     (BF, 128, 32, 2, 4, [700, 1000, 64, 64], [1, 130, 64, 1]), (HF, 64, 1024, 1, 6, [3000], [70]), (F32, 128, 64, 2, 4, [1500, 3], [40, 3]),
-    (BF, 256, 64, 2, 2, [2500], [33]), (BF, 64, 16, 1, 1, [16], [16]), (HF, 256, 16, 2, 1, [1300, 5], None),
+    (BF, 256, 64, 2, 2, [2500], [33]), (BF, 128, 32, 8, 16, [8 * i for i in range(32)], [min(8 * i, 16 if i % 3 else 1) for i in range(32)]),
+    (HF, 64, 16, 16, 2, [512] * 15 + [3], [256] * 15 + [3]), (HF, 128, 64, 8, 4, [70 + i for i in range(32)], [64 - i for i in range(32)]), (BF, 64, 16, 1, 1, [16], [16]), (HF, 256, 16, 2, 1, [1300, 5], None),
 ])
 def test_kv4_attention(dtype, dim, page, kv_heads, group, lens, news):
     q, cache, table, n, start = lb.attention_case(dtype, dim, page, kv_heads, group, lens, news, seed=len(lens))
@@ -258,27 +259,30 @@ def test_kv4_attention(dtype, dim, page, kv_heads, group, lens, news):
     assert torch.equal(out, again)
 
 
-@pytest.mark.parametrize("dtype", [BF, HF])
-def test_kv4_attention_masks(dtype):
-    q, cache, table, n, start = lb.attention_case(dtype, 64, 16, 1, 2, [40, 33], [5, 7])
+@pytest.mark.parametrize("dtype,many", [(BF, False), (HF, False), (BF, True), (HF, True)])
+def test_kv4_attention_masks(dtype, many):
+    """many: 64 key/value heads with 16 query heads each, 112 rows, 512 workgroups of 128 (the kernel for pieces of prompts)"""
+    lens, news = ([40, 33] * 4, [5, 7] * 4) if many else ([40, 33], [5, 7])
+    q, cache, table, n, start = lb.attention_case(dtype, 64, 16, 64 if many else 1, 16 if many else 2, lens, news)
     qd, td, nd, sd = _dev(q, table, n, start)
     cd = hx.Kv4Cache(*_dev(*cache))
     call = lambda c=cd, t=td, ln=nd, **kw: hx.kv4_attention(qd, c, t, ln, query_start=sd, **{"max_query_len": 7, **kw}).cpu()
-    lb.check_attention(call(causal=False), q, cache, table, n, start, causal=False)
-    lb.check_attention(call(scale=0.3, max_query_len=1), q, cache, table, n, start, scale=0.3)
-    few = torch.tensor([2, 33], dtype=torch.int32)
+    check = lambda *args, **kw: lb.check_attention(*args, p_terms=1 if many and dtype == BF else 2, **kw)
+    check(call(causal=False), q, cache, table, n, start, causal=False)
+    check(call(scale=0.3, max_query_len=7 if many else 1), q, cache, table, n, start, scale=0.3)
+    few = torch.tensor([2, 33] * (len(lens) // 2), dtype=torch.int32)
     out = call(ln=few.to(DEV))
-    lb.check_attention(out, q, cache, table, few, start)
+    check(out, q, cache, table, few, start)
     assert (out[:3] == 0).all()
     holes = table.clone()
     holes[0, 1], holes[1, 0] = 10**6, -1
-    lb.check_attention(call(t=holes.to(DEV)), q, cache, holes, n, start)
+    check(call(t=holes.to(DEV)), q, cache, holes, n, start)
     p, i = int(table[0, 38 // 16]), 38 % 16
     vs = cache[3].clone()
-    vs[p, 0, i // 4, 1, i % 4] = 255
+    vs[p, :, i // 4, 1, i % 4] = 255
     nan = (cache[0], cache[1], cache[2], vs)
     out = call(c=hx.Kv4Cache(*_dev(*nan)))
-    lb.check_attention(out, q, nan, table, n, start)
+    check(out, q, nan, table, n, start)
     assert torch.isnan(out[3:5, :, 32:]).all() and not torch.isnan(out[:3]).any()
 
 

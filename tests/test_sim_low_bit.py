@@ -171,6 +171,20 @@ def test_kv4_attention(dtype, dim, page, kv_heads, group, lens, news):
     lb.check_attention(out, q, cache, table, n, start, p_terms=lb.p_terms(dtype, dim, news, group))
 
 
+@pytest.mark.parametrize("dtype,dim,page,kv_heads,group,lens,news", [
+    (BF, 128, 16, 1, 4, [90, 20, 0, 3, 70], [33, 20, 0, 1, 4]),     # 132 rows: two workgroups; 80, none, 4 and 16 of them
+    (HF, 64, 64, 2, 1, [200], [130]), (HF, 128, 32, 1, 8, [40, 150], [9, 20]), (BF, 64, 16, 1, 3, [64, 129], [64, 1]),
+])
+def test_kv4_attention_many_rows(dtype, dim, page, kv_heads, group, lens, news):
+    """the kernel for pieces of prompts (a chip of one compute unit: it takes every batch with more than 64 rows)"""
+    q, cache, table, n, start = lb.attention_case(dtype, dim, page, kv_heads, group, lens, news)
+    with simlib.cus(1):
+        out = simops.kv4_attention(q, cache, table, n, start)
+        lb.check_attention(out, q, cache, table, n, start, p_terms=lb.p_terms(dtype, dim, news, group))
+        out = simops.kv4_attention(q, cache, table, n, start, causal=False, max_query=-(-65 // group))
+        lb.check_attention(out, q, cache, table, n, start, causal=False, p_terms=lb.p_terms(dtype, dim, news, group))
+
+
 @pytest.mark.parametrize("dtype,news", [(BF, None), (HF, [2, 40])])
 def test_kv4_attention_split_keys(dtype, news):
     """two splits of a long row (the table is wide enough), joined by the second kernel; rows behind the last sequence stay"""
@@ -186,38 +200,41 @@ def test_kv4_attention_split_keys(dtype, news):
         assert (out[42:].view(torch.uint8) == 0x11).all()
 
 
-def test_kv4_attention_masks():
+@pytest.mark.parametrize("many", [False, True])
+def test_kv4_attention_masks(many):
     """not causal; more new tokens than keys (rows without a key give zeros); a page that does not exist; lengths beyond the
     table; a max_query that is too small; NaN in a value that only later rows see"""
-    q, cache, table, n, start = lb.attention_case(BF, 64, 16, 1, 2, [40, 33], [5, 7])
-    out = simops.kv4_attention(q, cache, table, n, start, causal=False)
-    lb.check_attention(out, q, cache, table, n, start, causal=False)
-    out = simops.kv4_attention(q, cache, table, n, start, scale=0.3, max_query=1)
-    lb.check_attention(out, q, cache, table, n, start, scale=0.3)
-    few = torch.tensor([2, 33], dtype=torch.int32)
-    out = simops.kv4_attention(q, cache, table, few, start)
-    lb.check_attention(out, q, cache, table, few, start)
-    assert (out[:3] == 0).all()
-    holes = table.clone()
-    holes[0, 1], holes[1, 0] = 10**6, -1
-    out = simops.kv4_attention(q, cache, holes, n, start)
-    lb.check_attention(out, q, cache, holes, n, start)
-    far = torch.tensor([4000, 33], dtype=torch.int32)
-    full = torch.zeros(2, 3, dtype=torch.int32)
-    full[0], full[1] = table[0, :3], table[1, :3]
-    clamped = torch.tensor([48, 33], dtype=torch.int32)
-    kc, ks, vc, vs = (t.clone() for t in cache)
-    ks[ks == 255] = 120
-    vs[vs == 255] = 120
-    out = simops.kv4_attention(q, (kc, ks, vc, vs), full, far, start)
-    lb.check_attention(out, q, (kc, ks, vc, vs), full, clamped, start)
-    p, i = int(table[0, 38 // 16]), 38 % 16   # key 38: rows 3 and 4 of sequence 0 see it
-    vs2 = cache[3].clone()
-    vs2[p, 0, i // 4, 1, i % 4] = 255
-    nan = (cache[0], cache[1], cache[2], vs2)
-    out = simops.kv4_attention(q, nan, table, n, start)
-    lb.check_attention(out, q, nan, table, n, start)
-    assert torch.isnan(out[3:5, :, 32:]).all() and not torch.isnan(out[:3]).any() and not torch.isnan(out[:, :, :32]).any()
+    q, cache, table, n, start = lb.attention_case(BF, 64, 16, 1, 10 if many else 2, [40, 33], [5, 7])
+    check = lambda *args, **kw: lb.check_attention(*args, p_terms=1 if many else 2, **kw)
+    with simlib.cus(1 if many else 256):
+        out = simops.kv4_attention(q, cache, table, n, start, causal=False)
+        check(out, q, cache, table, n, start, causal=False)
+        out = simops.kv4_attention(q, cache, table, n, start, scale=0.3, max_query=7 if many else 1)
+        check(out, q, cache, table, n, start, scale=0.3)
+        few = torch.tensor([2, 33], dtype=torch.int32)
+        out = simops.kv4_attention(q, cache, table, few, start)
+        check(out, q, cache, table, few, start)
+        assert (out[:3] == 0).all()
+        holes = table.clone()
+        holes[0, 1], holes[1, 0] = 10**6, -1
+        out = simops.kv4_attention(q, cache, holes, n, start)
+        check(out, q, cache, holes, n, start)
+        far = torch.tensor([4000, 33], dtype=torch.int32)
+        full = torch.zeros(2, 3, dtype=torch.int32)
+        full[0], full[1] = table[0, :3], table[1, :3]
+        clamped = torch.tensor([48, 33], dtype=torch.int32)
+        kc, ks, vc, vs = (t.clone() for t in cache)
+        ks[ks == 255] = 120
+        vs[vs == 255] = 120
+        out = simops.kv4_attention(q, (kc, ks, vc, vs), full, far, start)
+        check(out, q, (kc, ks, vc, vs), full, clamped, start)
+        p, i = int(table[0, 38 // 16]), 38 % 16   # key 38: rows 3 and 4 of sequence 0 see it
+        vs2 = cache[3].clone()
+        vs2[p, 0, i // 4, 1, i % 4] = 255
+        nan = (cache[0], cache[1], cache[2], vs2)
+        out = simops.kv4_attention(q, nan, table, n, start)
+        check(out, q, nan, table, n, start)
+        assert torch.isnan(out[3:5, :, 32:]).all() and not torch.isnan(out[:3]).any() and not torch.isnan(out[:, :, :32]).any()
 
 
 def test_kv4_attention_no_pages():
