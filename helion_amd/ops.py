@@ -36,29 +36,28 @@ def _require_cuda(*tensors: torch.Tensor) -> None:
             raise RuntimeError("helion_amd ops run on the GPU only (HIP kernels); got a tensor on " + str(t.device))
 
 
-def _one_device(who: str, first: torch.Tensor, *rest: torch.Tensor | None) -> None:
-    for t in rest:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{who}: tensors on {first.device} and {t.device}")
+def _device_of(who: str, *tensors: torch.Tensor | None) -> int:
+    """Index of the GPU that all the tensors are on."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            _require_cuda(*tensors)
+            raise ValueError(f"{who}: tensors on {tensors[0].device} and {t.device}")
+    if index < 0:
+        _require_cuda(*tensors)
+    return index
 
 
-class _on:
-    """The device whose tensors a call works on is the current one inside the block (a launch goes to the current device,
-    the stream handle alone does not move it).  Costs one query where it already is."""
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
-    __slots__ = ("index", "old")
 
-    def __init__(self, device: torch.device):
-        self.index = device.index
-
-    def __enter__(self):
-        self.old = torch.cuda.current_device()
-        if self.old != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.old != self.index:
-            torch.cuda.set_device(self.old)
+def _launch(index: int, fn, *args) -> int:
+    """fn(*args, stream) on the current stream of GPU `index`, with that GPU current (a launch goes to the current device;
+    the stream handle alone does not move it)."""
+    if _current_device() == index:
+        return fn(*args, _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream)
+    with torch.cuda.device(index):
+        return fn(*args, torch.cuda.current_stream(index).cuda_stream)
 
 
 # ------------------------------------------------------------------------------ fp8 gemm
@@ -421,6 +420,10 @@ def _(q, k, v):
 
 
 # ------------------------------------------------------------------------------ rows to 8-bit integers, with and without a norm
+_CONTIGUOUS = torch.contiguous_format
+_FLOATS = (torch.float16, torch.bfloat16, torch.float32)
+
+
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x as [rows, width] with the elements of a row contiguous, without a copy where its strides allow that."""
     x = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
@@ -430,7 +433,7 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 
 
 def _check_rows(who: str, x: torch.Tensor) -> None:
-    if x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+    if x.dtype not in _FLOATS:
         raise TypeError(f"{who} expects float16/bfloat16/float32, got {x.dtype}")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= 65536:
         raise ValueError(f"{who} expects rows of 1 to 65536 elements, got shape {tuple(x.shape)}")
@@ -446,27 +449,25 @@ def _add_rms_norm_int8_impl(x: torch.Tensor, residual: torch.Tensor, weight: tor
 
 
 def _rms_norm_int8_any(x, residual, weight, eps):
-    _require_cuda(x, residual, weight)
+    index = _device_of("rms_norm_int8", x, residual, weight)
     _check_rows("rms_norm_int8", x)
-    width = x.shape[-1]
-    if weight.shape != (width,) or weight.dtype != x.dtype:
-        raise ValueError(f"rms_norm_int8: weight must be [{width}] of {x.dtype}, got {tuple(weight.shape)} of {weight.dtype}")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise ValueError(f"rms_norm_int8: residual must be {tuple(x.shape)} of {x.dtype}, got {tuple(residual.shape)} of {residual.dtype}")
-    _one_device("rms_norm_int8", x, residual, weight)
-    x2, dev = _rows(x), x.device
-    r2 = _rows(residual) if residual is not None else None
-    weight = weight.contiguous()
+    shape, dtype = x.shape, x.dtype
+    width = shape[-1]
+    if weight.shape != (width,) or weight.dtype != dtype:
+        raise ValueError(f"rms_norm_int8: weight must be [{width}] of {dtype}, got {tuple(weight.shape)} of {weight.dtype}")
+    x2, weight = _rows(x), weight.contiguous()
     rows = x2.shape[0]
-    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
-    scale = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=dev)
-    h = torch.empty(x.shape, dtype=x.dtype, device=dev) if residual is not None else None
+    q = torch.empty_like(x, dtype=torch.int8, memory_format=_CONTIGUOUS)
+    scale = x.new_empty((*shape[:-1], 1), dtype=torch.float32)
+    h = r2 = None
+    if residual is not None:
+        if residual.shape != shape or residual.dtype != dtype:
+            raise ValueError(f"rms_norm_int8: residual must be {tuple(shape)} of {dtype}, got {tuple(residual.shape)} of {residual.dtype}")
+        r2, h = _rows(residual), torch.empty_like(x, memory_format=_CONTIGUOUS)
     if rows:
-        with _on(dev):
-            rc = _lib.load().hx_rms_norm_int8(x2.data_ptr(), x2.stride(0), r2.data_ptr() if r2 is not None else None,
-                                              r2.stride(0) if r2 is not None else 0, weight.data_ptr(), eps,
-                                              h.data_ptr() if h is not None else None, q.data_ptr(), scale.data_ptr(), rows, width,
-                                              _DT[x.dtype], _stream_ptr(dev))
+        rc = _launch(index, _lib.load().hx_rms_norm_int8, x2.data_ptr(), x2.stride(0), r2.data_ptr() if r2 is not None else None,
+                     r2.stride(0) if r2 is not None else 0, weight.data_ptr(), eps, h.data_ptr() if h is not None else None, q.data_ptr(),
+                     scale.data_ptr(), rows, width, _DT[dtype])
         _lib.check(rc, "hx_rms_norm_int8")
     return q, scale, h
 
@@ -487,15 +488,14 @@ def _(x, residual, weight, eps):
 
 
 def _int8_quantize_impl(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    _require_cuda(x)
+    index = _device_of("int8_quantize_per_token", x)
     _check_rows("int8_quantize_per_token", x)
-    x2, dev = _rows(x), x.device
-    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
-    scale = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=dev)
+    x2 = _rows(x)
+    q = torch.empty_like(x, dtype=torch.int8, memory_format=_CONTIGUOUS)
+    scale = x.new_empty((*x.shape[:-1], 1), dtype=torch.float32)
     if x2.shape[0]:
-        with _on(dev):
-            rc = _lib.load().hx_int8_quantize_per_token(x2.data_ptr(), x2.stride(0), q.data_ptr(), scale.data_ptr(), x2.shape[0],
-                                                        x2.shape[1], _DT[x.dtype], _stream_ptr(dev))
+        rc = _launch(index, _lib.load().hx_int8_quantize_per_token, x2.data_ptr(), x2.stride(0), q.data_ptr(), scale.data_ptr(), x2.shape[0],
+                     x2.shape[1], _DT[x.dtype])
         _lib.check(rc, "hx_int8_quantize_per_token")
     return q, scale
 
@@ -511,7 +511,7 @@ def _(x):
 # ------------------------------------------------------------------------------ int8 gemm
 def _int8_gemm_impl(x: torch.Tensor, y: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor, bias: torch.Tensor | None,
                     out_dtype: torch.dtype) -> torch.Tensor:
-    _require_cuda(x, y, scale_a, scale_b, bias)
+    index = _device_of("int8_gemm", x, y, scale_a, scale_b, bias)
     if x.dtype != torch.int8 or y.dtype != torch.int8:
         raise TypeError(f"int8_gemm expects int8 operands, got {x.dtype} and {y.dtype}")
     if x.dim() != 2 or y.dim() != 2:
@@ -520,17 +520,17 @@ def _int8_gemm_impl(x: torch.Tensor, y: torch.Tensor, scale_a: torch.Tensor, sca
     k2, n = y.shape
     if k != k2:
         raise ValueError(f"int8_gemm: size mismatch {k} != {k2}")
-    if out_dtype not in (torch.float16, torch.bfloat16, torch.float32):
+    if out_dtype not in _FLOATS:
         raise TypeError(f"unsupported out_dtype {out_dtype}")
     if scale_a.dtype != torch.float32 or scale_b.dtype != torch.float32:
         raise TypeError("int8_gemm: scales must be float32")
     if scale_a.numel() != m or scale_b.numel() != n:
         raise ValueError(f"int8_gemm: scale_a must have {m} elements and scale_b {n}, got {scale_a.numel()} and {scale_b.numel()}")
-    if bias is not None and (bias.numel() != n or bias.dtype not in (torch.float16, torch.bfloat16, torch.float32)):
-        raise ValueError(f"int8_gemm: bias must be {n} float16/bfloat16/float32 elements, got {tuple(bias.shape)} of {bias.dtype}")
-    _one_device("int8_gemm", x, y, scale_a, scale_b, bias)
-    dev = x.device
-    out = torch.empty((m, n), dtype=out_dtype, device=dev)
+    if bias is not None:
+        if bias.numel() != n or bias.dtype not in _FLOATS:
+            raise ValueError(f"int8_gemm: bias must be {n} float16/bfloat16/float32 elements, got {tuple(bias.shape)} of {bias.dtype}")
+        bias = bias.contiguous()
+    out = x.new_empty((m, n), dtype=out_dtype)
     if m == 0 or n == 0:
         return out
     if k == 0:
@@ -538,20 +538,18 @@ def _int8_gemm_impl(x: torch.Tensor, y: torch.Tensor, scale_a: torch.Tensor, sca
     x = _rows(x)
     lda = x.stride(0) if m > 1 else k
     ldb_k = y.stride(0) if k > 1 else 1
-    ldb_n = y.stride(1) if n > 1 else max(k, 1)
+    ldb_n = y.stride(1) if n > 1 else k
     if ldb_k < 1 or ldb_n < 1:  # an expanded operand
         y = y.t().contiguous().t()
         ldb_k, ldb_n = 1, k
     scale_a, scale_b = scale_a.contiguous(), scale_b.contiguous()
-    bias = bias.contiguous() if bias is not None else None
     lib = _lib.load()
     xp, yp = x.data_ptr(), y.data_ptr()
-    with _on(dev):
-        ws_bytes = lib.hx_int8_gemm_workspace_bytes(m, n, k, lda, ldb_k, ldb_n, xp, yp)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-        rc = lib.hx_int8_gemm(xp, yp, out.data_ptr(), m, n, k, lda, ldb_k, ldb_n, n, scale_a.data_ptr(), scale_b.data_ptr(),
-                              bias.data_ptr() if bias is not None else None, _DT[bias.dtype] if bias is not None else 0, _DT[out_dtype],
-                              ws.data_ptr() if ws is not None else None, ws_bytes, _stream_ptr(dev))
+    ws_bytes = lib.hx_int8_gemm_workspace_bytes(m, n, k, lda, ldb_k, ldb_n, xp, yp)
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+    rc = _launch(index, lib.hx_int8_gemm, xp, yp, out.data_ptr(), m, n, k, lda, ldb_k, ldb_n, n, scale_a.data_ptr(), scale_b.data_ptr(),
+                 bias.data_ptr() if bias is not None else None, _DT[bias.dtype] if bias is not None else 0, _DT[out_dtype],
+                 ws.data_ptr() if ws is not None else None, ws_bytes)
     _lib.check(rc, "hx_int8_gemm")
     return out
 
@@ -567,18 +565,19 @@ def _(x, y, scale_a, scale_b, bias, out_dtype):
 # ------------------------------------------------------------------------------ key/value cache in 4 bits
 def _check_cache(who: str, kc: torch.Tensor, ks: torch.Tensor, vc: torch.Tensor, vs: torch.Tensor) -> tuple[int, int, int, int]:
     """(pages, heads, page, head_dim) of a cache whose four tensors fit together."""
-    if any(t.dtype != torch.uint8 for t in (kc, ks, vc, vs)):
+    u8 = torch.uint8
+    if kc.dtype != u8 or ks.dtype != u8 or vc.dtype != u8 or vs.dtype != u8:
         raise TypeError(f"{who}: the cache's tensors must be uint8")
     if kc.dim() != 4:
         raise ValueError(f"{who}: k must be [pages, heads, page, head_dim / 2], got {tuple(kc.shape)}")
     pages, heads, page, half = kc.shape
-    d = 2 * half
+    d, s = 2 * half, half // 16
     if d not in (64, 128, 256):
         raise ValueError(f"{who}: head_dim must be 64, 128 or 256, got {d}")
     if page < 16 or page > 1024 or page & (page - 1):
         raise ValueError(f"{who}: pages hold a power of two from 16 to 1024 tokens, got {page}")
-    if (ks.shape != (pages, heads, page, d // 32) or vc.shape != (pages, heads, page // 4, 16, 4, d // 32)
-            or vs.shape != (pages, heads, page // 4, d // 32, 4)):
+    if (ks.shape != (pages, heads, page, s) or vc.shape != (pages, heads, page // 4, 16, 4, s)
+            or vs.shape != (pages, heads, page // 4, s, 4)):
         raise ValueError(f"{who}: the cache's tensors do not fit together: {tuple(kc.shape)} {tuple(ks.shape)} {tuple(vc.shape)} {tuple(vs.shape)}")
     if not (kc.is_contiguous() and ks.is_contiguous() and vc.is_contiguous() and vs.is_contiguous()):
         raise ValueError(f"{who}: the cache's tensors must be contiguous")
@@ -598,22 +597,20 @@ def _heads_of(t: torch.Tensor) -> torch.Tensor:
 
 def _kv4_write_impl(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor, k: torch.Tensor,
                     v: torch.Tensor, slots: torch.Tensor) -> None:
-    _require_cuda(k_codes, k_scales, v_codes, v_scales, k, v, slots)
+    index = _device_of("kv4_write", k_codes, k_scales, v_codes, v_scales, k, v, slots)
     pages, heads, page, d = _check_cache("kv4_write", k_codes, k_scales, v_codes, v_scales)
-    if k.dtype not in (torch.float16, torch.bfloat16, torch.float32) or v.dtype != k.dtype:
+    if k.dtype not in _FLOATS or v.dtype != k.dtype:
         raise TypeError(f"kv4_write expects k and v of one dtype out of float16, bfloat16, float32; got {k.dtype} and {v.dtype}")
     if k.dim() != 3 or k.shape[1:] != (heads, d) or v.shape != k.shape:
         raise ValueError(f"kv4_write: k and v must be [tokens, {heads}, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
     tokens = k.shape[0]
     slots = _check_slots("kv4_write", slots, tokens)
-    _one_device("kv4_write", k_codes, k_scales, v_codes, v_scales, k, v, slots)
     if tokens == 0:
         return
-    k, v, dev = _heads_of(k), _heads_of(v), k.device
-    with _on(dev):
-        rc = _lib.load().hx_kv4_write(k.data_ptr(), v.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
-                                      v_scales.data_ptr(), slots.data_ptr(), int(slots.dtype == torch.int64), tokens, heads, d, pages,
-                                      page, k.stride(0), k.stride(1), v.stride(0), v.stride(1), _DT[k.dtype], _stream_ptr(dev))
+    k, v = _heads_of(k), _heads_of(v)
+    rc = _launch(index, _lib.load().hx_kv4_write, k.data_ptr(), v.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+                 v_scales.data_ptr(), slots.data_ptr(), int(slots.dtype == torch.int64), tokens, heads, d, pages, page, k.stride(0),
+                 k.stride(1), v.stride(0), v.stride(1), _DT[k.dtype])
     _lib.check(rc, "hx_kv4_write")
 
 
@@ -627,20 +624,16 @@ def _(k_codes, k_scales, v_codes, v_scales, k, v, slots):
 
 def _kv4_read_impl(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor, slots: torch.Tensor,
                    dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
-    _require_cuda(k_codes, k_scales, v_codes, v_scales, slots)
+    index = _device_of("kv4_read", k_codes, k_scales, v_codes, v_scales, slots)
     pages, heads, page, d = _check_cache("kv4_read", k_codes, k_scales, v_codes, v_scales)
-    if dtype not in (torch.float16, torch.bfloat16, torch.float32):
+    if dtype not in _FLOATS:
         raise TypeError(f"kv4_read: dtype must be float16, bfloat16 or float32, got {dtype}")
     slots = _check_slots("kv4_read", slots)
-    _one_device("kv4_read", k_codes, k_scales, v_codes, v_scales, slots)
-    tokens, dev = slots.shape[0], k_codes.device
-    k = torch.empty((tokens, heads, d), dtype=dtype, device=dev)
-    v = torch.empty((tokens, heads, d), dtype=dtype, device=dev)
+    tokens = slots.shape[0]
+    k, v = k_codes.new_empty((tokens, heads, d), dtype=dtype), k_codes.new_empty((tokens, heads, d), dtype=dtype)
     if tokens:
-        with _on(dev):
-            rc = _lib.load().hx_kv4_read(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
-                                         slots.data_ptr(), int(slots.dtype == torch.int64), k.data_ptr(), v.data_ptr(), tokens, heads, d,
-                                         pages, page, _DT[dtype], _stream_ptr(dev))
+        rc = _launch(index, _lib.load().hx_kv4_read, k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
+                     slots.data_ptr(), int(slots.dtype == torch.int64), k.data_ptr(), v.data_ptr(), tokens, heads, d, pages, page, _DT[dtype])
         _lib.check(rc, "hx_kv4_read")
     return k, v
 
@@ -655,51 +648,60 @@ def _(k_codes, k_scales, v_codes, v_scales, slots, dtype):
 
 
 # ------------------------------------------------------------------------------ attention over it
-def _kv4_attention_into(out: torch.Tensor, q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
+def _kv4_attention_into(out: torch.Tensor | None, q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
                         v_scales: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, query_start: torch.Tensor | None,
-                        max_query_len: int, scale: float, causal: bool) -> None:
-    _require_cuda(out, q, k_codes, k_scales, v_codes, v_scales, block_table, seq_lens, query_start)
+                        max_query_len: int, scale: float, causal: bool) -> torch.Tensor:
+    index = _device_of("kv4_attention", q, out, k_codes, k_scales, v_codes, v_scales, block_table, seq_lens, query_start)
     pages, kv_heads, page, d = _check_cache("kv4_attention", k_codes, k_scales, v_codes, v_scales)
-    if q.dtype not in (torch.float16, torch.bfloat16, torch.float32):
-        raise TypeError(f"kv4_attention expects a float16, bfloat16 or float32 q, got {q.dtype}")
+    dtype, i32 = q.dtype, torch.int32
+    if dtype not in _FLOATS:
+        raise TypeError(f"kv4_attention expects a float16, bfloat16 or float32 q, got {dtype}")
     if q.dim() != 3 or q.shape[2] != d or kv_heads < 1 or q.shape[1] % kv_heads:
         raise ValueError(f"kv4_attention: q must be [tokens, a multiple of {kv_heads} heads, {d}], got {tuple(q.shape)}")
     tokens, heads, _ = q.shape
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32 or seq_lens.dim() != 1:
+    if block_table.dim() != 2 or block_table.dtype != i32 or seq_lens.dtype != i32 or seq_lens.dim() != 1:
         raise ValueError("kv4_attention: block_table must be [sequences, pages] and seq_lens [sequences], both int32")
     batch, width = block_table.shape
     if seq_lens.shape[0] != batch:
         raise ValueError(f"kv4_attention: {seq_lens.shape[0]} lengths for {batch} rows of the block table")
-    if query_start is not None and (query_start.dtype != torch.int32 or query_start.shape != (batch + 1,)):
-        raise ValueError(f"kv4_attention: query_start must be [{batch + 1}] int32, got {tuple(query_start.shape)} of {query_start.dtype}")
-    if query_start is None and tokens != batch:
-        raise ValueError(f"kv4_attention: without query_start q holds one token for each of the {batch} sequences, got {tokens}")
-    if max_query_len < 1:
-        raise ValueError(f"kv4_attention: max_query_len must be at least 1, got {max_query_len}")
-    if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
-        raise ValueError(f"kv4_attention: out must be contiguous {tuple(q.shape)} of {q.dtype}")
-    _one_device("kv4_attention", out, q, k_codes, k_scales, v_codes, v_scales, block_table, seq_lens, query_start)
+    if query_start is None:
+        max_query_len = 1
+        if tokens != batch:
+            raise ValueError(f"kv4_attention: without query_start q holds one token for each of the {batch} sequences, got {tokens}")
+    else:
+        if query_start.dtype != i32 or query_start.shape != (batch + 1,):
+            raise ValueError(f"kv4_attention: query_start must be [{batch + 1}] int32, got {tuple(query_start.shape)} of {query_start.dtype}")
+        if max_query_len < 1:
+            raise ValueError(f"kv4_attention: max_query_len must be at least 1, got {max_query_len}")
+        query_start = query_start.contiguous()
+    if out is None:
+        out = torch.empty_like(q, memory_format=_CONTIGUOUS)
+    elif out.shape != q.shape or out.dtype != dtype or not out.is_contiguous():
+        raise ValueError(f"kv4_attention: out must be contiguous {tuple(q.shape)} of {dtype}")
     if tokens == 0 or heads == 0 or batch == 0:
-        return
-    q, dev = _heads_of(q), q.device
+        return out
+    q = _heads_of(q)
     if width > 1 and block_table.stride(1) != 1 or batch > 1 and block_table.stride(0) < width:
         block_table = block_table.contiguous()
     seq_lens = seq_lens.contiguous()
-    query_start = query_start.contiguous() if query_start is not None else None
     lib = _lib.load()
-    with _on(dev):
-        ws_bytes = lib.hx_kv4_attention_workspace_bytes(tokens, batch, heads, kv_heads, d, page, width,
-                                                        max_query_len if query_start is not None else 1, _DT[q.dtype])
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-        rc = lib.hx_kv4_attention(q.data_ptr(), q.stride(0), q.stride(1), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
-                                  v_scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr(),
-                                  query_start.data_ptr() if query_start is not None else None, out.data_ptr(), tokens, batch, heads,
-                                  kv_heads, d, pages, page, width, max_query_len, scale, int(causal), _DT[q.dtype],
-                                  ws.data_ptr() if ws is not None else None, ws_bytes, _stream_ptr(dev))
+    ws_bytes = lib.hx_kv4_attention_workspace_bytes(tokens, batch, heads, kv_heads, d, page, width, max_query_len, _DT[dtype])
+    ws = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+    rc = _launch(index, lib.hx_kv4_attention, q.data_ptr(), q.stride(0), q.stride(1), k_codes.data_ptr(), k_scales.data_ptr(),
+                 v_codes.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr(),
+                 query_start.data_ptr() if query_start is not None else None, out.data_ptr(), tokens, batch, heads, kv_heads, d, pages, page,
+                 width, max_query_len, scale, causal, _DT[dtype], ws.data_ptr() if ws is not None else None, ws_bytes)
     _lib.check(rc, "hx_kv4_attention")
+    return out
 
 
-kv4_attention_out_op = torch.library.custom_op("helion_amd::kv4_attention_out", mutates_args=("out",))(_kv4_attention_into)
+def _kv4_attention_out_impl(out: torch.Tensor, q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
+                            v_scales: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, query_start: torch.Tensor | None,
+                            max_query_len: int, scale: float, causal: bool) -> None:
+    _kv4_attention_into(out, q, k_codes, k_scales, v_codes, v_scales, block_table, seq_lens, query_start, max_query_len, scale, causal)
+
+
+kv4_attention_out_op = torch.library.custom_op("helion_amd::kv4_attention_out", mutates_args=("out",))(_kv4_attention_out_impl)
 
 
 @kv4_attention_out_op.register_fake
@@ -710,9 +712,7 @@ def _(out, q, k_codes, k_scales, v_codes, v_scales, block_table, seq_lens, query
 def _kv4_attention_impl(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor,
                         block_table: torch.Tensor, seq_lens: torch.Tensor, query_start: torch.Tensor | None, max_query_len: int,
                         scale: float, causal: bool) -> torch.Tensor:
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _kv4_attention_into(out, q, k_codes, k_scales, v_codes, v_scales, block_table, seq_lens, query_start, max_query_len, scale, causal)
-    return out
+    return _kv4_attention_into(None, q, k_codes, k_scales, v_codes, v_scales, block_table, seq_lens, query_start, max_query_len, scale, causal)
 
 
 kv4_attention_op = torch.library.custom_op("helion_amd::kv4_attention", mutates_args=())(_kv4_attention_impl)
@@ -739,11 +739,26 @@ cast_e4m3_x3_call = _caller(_cast_e4m3_x3_impl, cast_e4m3_x3_op)
 fp8_quantize_call = _caller(_fp8_quantize_impl, fp8_quantize_op)
 matmul_call = _caller(_matmul_impl, matmul_op)
 attention_call = _caller(_attention_impl, attention_op)
-rms_norm_int8_call = _caller(_rms_norm_int8_impl, rms_norm_int8_op)
-add_rms_norm_int8_call = _caller(_add_rms_norm_int8_impl, add_rms_norm_int8_op)
-int8_quantize_call = _caller(_int8_quantize_impl, int8_quantize_op)
-int8_gemm_call = _caller(_int8_gemm_impl, int8_gemm_op)
-kv4_write_call = _caller(_kv4_write_impl, kv4_write_op)
-kv4_read_call = _caller(_kv4_read_impl, kv4_read_op)
-kv4_attention_call = _caller(_kv4_attention_impl, kv4_attention_op)
-kv4_attention_out_call = _caller(_kv4_attention_into, kv4_attention_out_op)
+
+
+def _light_caller(impl, op, tensors):
+    """As _caller, for calls whose first `tensors` arguments are the tensors (or None): these are all it looks at."""
+    def call(*args):
+        if not torch.compiler.is_compiling():
+            for t in args[:tensors]:
+                if t is not None and (type(t) is not torch.Tensor or not t.is_cuda):
+                    break
+            else:
+                return impl(*args)
+        return op(*args)
+    return call
+
+
+rms_norm_int8_call = _light_caller(_rms_norm_int8_impl, rms_norm_int8_op, 2)
+add_rms_norm_int8_call = _light_caller(_add_rms_norm_int8_impl, add_rms_norm_int8_op, 3)
+int8_quantize_call = _light_caller(_int8_quantize_impl, int8_quantize_op, 1)
+int8_gemm_call = _light_caller(_int8_gemm_impl, int8_gemm_op, 5)
+kv4_write_call = _light_caller(_kv4_write_impl, kv4_write_op, 7)
+kv4_read_call = _light_caller(_kv4_read_impl, kv4_read_op, 5)
+kv4_attention_call = _light_caller(_kv4_attention_impl, kv4_attention_op, 8)
+kv4_attention_out_call = _light_caller(_kv4_attention_out_impl, kv4_attention_out_op, 9)
