@@ -1,9 +1,11 @@
 // Writing tokens into the 4-bit key/value cache and reading them back (format and layout: kv4_format.h).
 //
-// Both are streams: write reads k and v once and writes D/2 + D/32 bytes per token, head and side; read does the
-// opposite.  A lane holds eight consecutive elements of one head of one token: 16 bytes of a 16-bit type, one dword of
+// Both are streams, bound by memory: write reads k and v once and writes D/2 + D/32 bytes per token, head and side; read
+// does the opposite.  A lane holds eight consecutive elements of one head of one token: 16 bytes of a 16-bit type, one dword of
 // codes; the four lanes of a 32-element block find its maximum with two shuffles.  A wave takes several consecutive
 // tokens of one head, so that where their slots are consecutive too (a prompt) the codes of the wave fill whole lines.
+// Loads of eight heads are on their way at once, and what is read once goes past the caches: 16384 tokens of 8 heads of 128
+// written and read back 68 -> 39 us, 172 MB at 4.5 TB/s.
 #include "hx_common.h"
 #include "kv4_format.h"
 
@@ -11,6 +13,8 @@
 
 #define KV4_THREADS 256
 #define KV4_BUCKETS 1024
+#define KV4_AHEAD 8          // heads whose loads are on their way before the first is worked on
+#define KV4_TURN (1 << 15)   // tokens written by one launch
 
 template <int DT>
 struct KvT;
@@ -50,43 +54,51 @@ __device__ __forceinline__ void kv4_place(int in_page, int l, int* code, int* sc
   }
 }
 
-// Which of the workgroup's tokens (t0 .. t0+63) are overtaken by a later token with the same slot: bit j of the result.
-// Their slots go into a small table; the slots of all later tokens are looked up in it.  The later one wins, whatever
+// Which of the workgroup's tokens (t0 .. t0+n-1, n up to 32) are overtaken by a later token with the same slot: bit j of the result.
+// Their slots go into a small table; the slots of all later tokens of the launch are looked up in it.  The later one wins, whatever
 // order the workgroups run in.
 template <typename I>
-__device__ uint64_t kv4_overtaken(const I* __restrict__ slots, long tokens, long capacity, long t0, int n) {
-  __shared__ uint32_t table[2][KV4_BUCKETS];
-  __shared__ uint32_t dead[2];
-  __shared__ I mine[64];
-  for (int i = threadIdx.x; i < 2 * KV4_BUCKETS; i += KV4_THREADS) (&table[0][0])[i] = 0;
-  if (threadIdx.x < 2) dead[threadIdx.x] = 0;
+__device__ uint32_t kv4_overtaken(const I* __restrict__ slots, long tokens, long capacity, long t0, int n) {
+  __shared__ uint32_t table[KV4_BUCKETS];
+  __shared__ uint32_t dead;
+  __shared__ I mine[32];
+  for (int i = threadIdx.x; i < KV4_BUCKETS; i += KV4_THREADS) table[i] = 0;
+  if (threadIdx.x == 0) dead = 0;
   if ((int)threadIdx.x < n) mine[threadIdx.x] = slots[t0 + threadIdx.x];
   __syncthreads();
   if ((int)threadIdx.x < n && mine[threadIdx.x] >= 0 && (long)mine[threadIdx.x] < capacity)
-    atomicOr(&table[threadIdx.x >> 5][(uint32_t)mine[threadIdx.x] % KV4_BUCKETS], 1u << (threadIdx.x & 31));
+    atomicOr(&table[(uint32_t)mine[threadIdx.x] % KV4_BUCKETS], 1u << threadIdx.x);
   __syncthreads();
-  for (long t = t0 + 1 + threadIdx.x; t < tokens; t += KV4_THREADS) {
-    const I s = slots[t];
-    const uint32_t b = (uint32_t)s % KV4_BUCKETS;
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      uint32_t m = table[w][b];
-      while (m) {
-        const int j = __builtin_ctz(m);
-        m &= m - 1;
-        if (mine[32 * w + j] == s && t0 + 32 * w + j < t) atomicOr(&dead[w], 1u << j);
-      }
+  auto look = [&](I s, long t) {
+    uint32_t m = table[(uint32_t)s % KV4_BUCKETS];
+    if (m) m &= ~*(volatile uint32_t*)&dead;  // (what another lane has found already need not be found again)
+    while (m) {
+      const int j = __builtin_ctz(m);
+      m &= m - 1;
+      if (mine[j] == s && t0 + j < t) atomicOr(&dead, 1u << j);
     }
+  };
+  constexpr int U = 8;  // slots on their way per lane: the look through a long prompt is a chain of loads otherwise
+  long at = t0 + 1 + threadIdx.x;
+  for (; at + (U - 1) * KV4_THREADS < tokens; at += U * KV4_THREADS) {
+    I s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) s[u] = slots[at + u * KV4_THREADS];
+#pragma unroll
+    for (int u = 0; u < U; ++u) look(s[u], at + u * KV4_THREADS);
   }
+  for (; at < tokens; at += KV4_THREADS) look(slots[at], at);
   __syncthreads();
-  return dead[0] | ((uint64_t)dead[1] << 32);
+  return dead;
 }
 
+template <typename T>
+struct Kv4Raw {
+  typedef T V __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+};
 template <int D, bool VALUES, typename T>
-__device__ __forceinline__ void kv4_put(const T* __restrict__ src, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int in_page,
-                                        int l) {
-  typedef T Tv __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-  const Tv raw = *(const Tv*)(src + 8 * l);
+__device__ __forceinline__ void kv4_put(const typename Kv4Raw<T>::V raw, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                        int in_page, int l) {
   float f[8];
   uint32_t top = 0;
 #pragma unroll
@@ -118,7 +130,7 @@ __device__ __forceinline__ void kv4_put(const T* __restrict__ src, uint8_t* __re
 
 // Both kernels: grid (groups of `per` tokens, groups of `hb` heads, keys / values); a workgroup takes 256 / (D/8) tokens of
 // one head at a time.
-template <int DT, int D, typename I>
+template <int DT, int D, int A, typename I>
 __global__ __launch_bounds__(KV4_THREADS) void hx_kv4_write_kernel(Kv4Rows rows, Kv4Ptrs cache, const I* __restrict__ slots, long tokens,
                                                                   int heads, int page_shift, long capacity, int per, int hb) {
   typedef typename KvT<DT>::T T;
@@ -127,36 +139,42 @@ __global__ __launch_bounds__(KV4_THREADS) void hx_kv4_write_kernel(Kv4Rows rows,
   const long t0 = (long)blockIdx.x * per;
   const int n = (int)min((long)per, tokens - t0);
   const int h0 = blockIdx.y * hb, h1 = min(h0 + hb, heads);
-  const uint64_t dead = kv4_overtaken<I>(slots, tokens, capacity, t0, n);
+  const uint32_t dead = kv4_overtaken<I>(slots, tokens, capacity, t0, n);
   const int side = blockIdx.z, l = threadIdx.x % L, pm = (1 << page_shift) - 1;
   for (int j = threadIdx.x / L; j < n; j += RPS) {
     const long slot = (long)slots[t0 + j];
     if (slot < 0 || slot >= capacity || ((dead >> j) & 1)) continue;
-    const T* src = (const T*)rows.p[side] + (t0 + j) * rows.token_stride[side];
-    for (int h = h0; h < h1; ++h) {
-      const long at = ((slot >> page_shift) * heads + h) << page_shift;  // tokens in front of this page of this head
-      uint8_t* codes = (uint8_t*)cache.codes[side] + at * (D / 2);
-      uint8_t* scales = (uint8_t*)cache.scales[side] + at * (D / 32);
-      if (side == 0) kv4_put<D, false>(src + h * rows.head_stride[side], codes, scales, (int)(slot & pm), l);
-      else kv4_put<D, true>(src + h * rows.head_stride[side], codes, scales, (int)(slot & pm), l);
+    const T* src = (const T*)rows.p[side] + (t0 + j) * rows.token_stride[side] + 8 * l;
+    for (int h = h0; h < h1; h += A) {
+      typename Kv4Raw<T>::V raw[A];
+#pragma unroll
+      for (int u = 0; u < A; ++u)
+        raw[u] = __builtin_nontemporal_load((const typename Kv4Raw<T>::V*)(src + min(h + u, h1 - 1) * rows.head_stride[side]));
+#pragma unroll
+      for (int u = 0; u < A; ++u) {
+        if (h + u >= h1) break;
+        const long at = ((slot >> page_shift) * heads + h + u) << page_shift;  // tokens in front of this page of this head
+        uint8_t* codes = (uint8_t*)cache.codes[side] + at * (D / 2);
+        uint8_t* scales = (uint8_t*)cache.scales[side] + at * (D / 32);
+        if (side == 0) kv4_put<D, false, T>(raw[u], codes, scales, (int)(slot & pm), l);
+        else kv4_put<D, true, T>(raw[u], codes, scales, (int)(slot & pm), l);
+      }
     }
   }
 }
 
-// eight elements of one token of one head as fp32
+// eight elements of one token of one head: dword of codes and byte of scale
 template <int D, bool VALUES>
-__device__ __forceinline__ void kv4_get(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int in_page, int l, float (&f)[8]) {
+__device__ __forceinline__ void kv4_get(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int in_page, int l, uint32_t* c,
+                                        uint32_t* byte) {
   int at_code, at_scale;
   kv4_place<D, VALUES>(in_page, l, &at_code, &at_scale);
-  uint32_t c;
-  if (VALUES && D == 64) c = *(const uint16_t*)(codes + at_code) | ((uint32_t) * (const uint16_t*)(codes + at_code + 8) << 16);
-  else c = *(const uint32_t*)(codes + at_code);
-  const float s = kv4_scale(scales[at_scale]);
-  const v2f p0 = kv4_pair_f32<0>(c, s), p1 = kv4_pair_f32<1>(c, s), p2 = kv4_pair_f32<2>(c, s), p3 = kv4_pair_f32<3>(c, s);
-  f[0] = p0[0], f[1] = p0[1], f[2] = p1[0], f[3] = p1[1], f[4] = p2[0], f[5] = p2[1], f[6] = p3[0], f[7] = p3[1];
+  if (VALUES && D == 64) *c = *(const uint16_t*)(codes + at_code) | ((uint32_t) * (const uint16_t*)(codes + at_code + 8) << 16);
+  else *c = *(const uint32_t*)(codes + at_code);
+  *byte = scales[at_scale];
 }
 
-template <int DT, int D, typename I>
+template <int DT, int D, int A, typename I>
 __global__ __launch_bounds__(KV4_THREADS) void hx_kv4_read_kernel(Kv4Ptrs cache, Kv4Ptrs out, const I* __restrict__ slots, long tokens,
                                                                  int heads, int page_shift, long capacity, int per, int hb) {
   typedef typename KvT<DT>::T T;
@@ -170,20 +188,28 @@ __global__ __launch_bounds__(KV4_THREADS) void hx_kv4_read_kernel(Kv4Ptrs cache,
   for (int j = threadIdx.x / L; j < n; j += RPS) {
     const long slot = (long)slots[t0 + j];
     const bool there = slot >= 0 && slot < capacity;
-    T* dst = (T*)out.codes[side] + (t0 + j) * heads * D;
-    for (int h = h0; h < h1; ++h) {
-      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (there) {
-        const long at = ((slot >> page_shift) * heads + h) << page_shift;
+    T* dst = (T*)out.codes[side] + (t0 + j) * heads * D + 8 * l;
+    for (int h = h0; h < h1; h += A) {
+      uint32_t c[A], byte[A];
+#pragma unroll
+      for (int u = 0; u < A; ++u) {
+        c[u] = 0, byte[u] = 127;
+        if (!there) continue;
+        const long at = ((slot >> page_shift) * heads + min(h + u, h1 - 1)) << page_shift;
         const uint8_t* codes = (const uint8_t*)cache.codes[side] + at * (D / 2);
         const uint8_t* scales = (const uint8_t*)cache.scales[side] + at * (D / 32);
-        if (side == 0) kv4_get<D, false>(codes, scales, (int)(slot & pm), l, f);
-        else kv4_get<D, true>(codes, scales, (int)(slot & pm), l, f);
+        if (side == 0) kv4_get<D, false>(codes, scales, (int)(slot & pm), l, &c[u], &byte[u]);
+        else kv4_get<D, true>(codes, scales, (int)(slot & pm), l, &c[u], &byte[u]);
       }
-      Tv v;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (T)f[e];
-      *(Tv*)(dst + h * D + 8 * l) = v;
+      for (int u = 0; u < A; ++u) {
+        if (h + u >= h1) break;
+        const float s = kv4_scale(byte[u]);
+        const v2f p0 = kv4_pair_f32<0>(c[u], s), p1 = kv4_pair_f32<1>(c[u], s), p2 = kv4_pair_f32<2>(c[u], s), p3 = kv4_pair_f32<3>(c[u], s);
+        Tv v;
+        v[0] = (T)p0[0], v[1] = (T)p0[1], v[2] = (T)p1[0], v[3] = (T)p1[1], v[4] = (T)p2[0], v[5] = (T)p2[1], v[6] = (T)p3[0], v[7] = (T)p3[1];
+        __builtin_nontemporal_store(v, (Tv*)(dst + (long)(h + u) * D));
+      }
     }
   }
 }
@@ -221,10 +247,14 @@ int kv4_check_cache(const char* who, const void* kc, const void* ks, const void*
 static int kv4_shift(int64_t page) { return __builtin_ctzll((unsigned long long)page); }
 
 template <typename F>
-static void kv4_pick(int dt, int64_t D, int wide, F&& f) {
+static void kv4_pick(int dt, int64_t D, int hb, int wide, F&& f) {
   auto by_i = [&](auto dtc, auto dc) {
-    if (wide) f(dtc, dc, (int64_t)0);
-    else f(dtc, dc, (int32_t)0);
+    auto by_a = [&](auto i) {
+      if (hb >= 4) f(dtc, dc, std::integral_constant<int, KV4_AHEAD>{}, i);
+      else f(dtc, dc, std::integral_constant<int, 1>{}, i);
+    };
+    if (wide) by_a((int64_t)0);
+    else by_a((int32_t)0);
   };
   auto by_d = [&](auto dtc) {
     if (D == 64) by_i(dtc, std::integral_constant<int, 64>{});
@@ -260,15 +290,16 @@ static int kv4_check_rows(const char* who, int64_t tokens, int dt, const void* s
   return 0;
 }
 
-// Tokens and heads per workgroup: 64 tokens and all heads keep the look for later tokens of the same slot (every workgroup
-// reads the slots behind its own) small next to the data; few tokens are spread over more workgroups instead.
+// Tokens and heads per workgroup: 32 tokens and all heads keep the look for later tokens of the same slot (every workgroup
+// reads the slots behind its own: 3 of the 39 us above) small next to the data, at 64 there are too few workgroups for the
+// chip (42 us), at 16 too much looking (41); few tokens are spread over more workgroups, with their heads one by one.
 struct Kv4Grid {
   int per, hb;
   unsigned x, y;
 };
 static Kv4Grid kv4_grid(int64_t tokens, int64_t heads, int64_t D) {
   Kv4Grid g;
-  g.per = tokens >= 4096 ? 64 : D == 64 ? 32 : 16;
+  g.per = tokens >= 4096 || D == 64 ? 32 : 16;
   g.x = (unsigned)((tokens + g.per - 1) / g.per);
   g.hb = (int)heads;
   while (g.hb > 1 && (long)g.x * ((heads + g.hb - 1) / g.hb) < hx_cu_count()) g.hb = (g.hb + 1) / 2;
@@ -300,15 +331,23 @@ extern "C" int hx_kv4_write(const void* k, const void* v, void* k_codes, void* k
     hx_set_error("hx_kv4_write: k and v must be aligned to their elements");
     return HX_ERR_UNSUPPORTED;
   }
-  const Kv4Grid g = kv4_grid(tokens, heads, D);
-  Kv4Rows rows = {{k, v}, {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride}};
+  // One launch after the other for very many tokens: the look for later ones stays within a launch, and a later launch
+  // overwrites an earlier one, so that the work stays proportional to the tokens.
+  const int64_t es = dtype == HX_F32 ? 4 : 2;
   Kv4Ptrs cache = {{k_codes, v_codes}, {k_scales, v_scales}};
-  kv4_pick(dtype, D, slots_are_int64, [&](auto dtc, auto dc, auto i) {
-    typedef decltype(i) I;
-    hx_launch(hx_kv4_write_kernel<decltype(dtc)::value, decltype(dc)::value, I>,
-              dim3(g.x, g.y, 2), dim3(KV4_THREADS), 0, (hipStream_t)stream, rows, cache, (const I*)slots, (long)tokens, (int)heads,
-              kv4_shift(page), (long)(pages * page), g.per, g.hb);
-  });
+  for (int64_t first = 0; first < tokens; first += KV4_TURN) {
+    const int64_t n = tokens - first < KV4_TURN ? tokens - first : KV4_TURN;
+    const Kv4Grid g = kv4_grid(n, heads, D);
+    Kv4Rows rows = {{(const char*)k + first * k_token_stride * es, (const char*)v + first * v_token_stride * es},
+                    {k_token_stride, v_token_stride},
+                    {k_head_stride, v_head_stride}};
+    kv4_pick(dtype, D, g.hb, slots_are_int64, [&](auto dtc, auto dc, auto a, auto i) {
+      typedef decltype(i) I;
+      hx_launch(hx_kv4_write_kernel<decltype(dtc)::value, decltype(dc)::value, decltype(a)::value, I>, dim3(g.x, g.y, 2),
+                dim3(KV4_THREADS), 0, (hipStream_t)stream, rows, cache, (const I*)slots + first, (long)n, (int)heads, kv4_shift(page),
+                (long)(pages * page), g.per, g.hb);
+    });
+  }
   return kv4_status("hx_kv4_write");
 }
 
@@ -328,9 +367,9 @@ extern "C" int hx_kv4_read(const void* k_codes, const void* k_scales, const void
   }
   Kv4Ptrs cache = {{(void*)k_codes, (void*)v_codes}, {(void*)k_scales, (void*)v_scales}}, out = {{k, v}, {nullptr, nullptr}};
   const Kv4Grid g = kv4_grid(tokens, heads, D);
-  kv4_pick(dtype, D, slots_are_int64, [&](auto dtc, auto dc, auto i) {
+  kv4_pick(dtype, D, g.hb, slots_are_int64, [&](auto dtc, auto dc, auto a, auto i) {
     typedef decltype(i) I;
-    hx_launch(hx_kv4_read_kernel<decltype(dtc)::value, decltype(dc)::value, I>, dim3(g.x, g.y, 2), dim3(KV4_THREADS), 0,
+    hx_launch(hx_kv4_read_kernel<decltype(dtc)::value, decltype(dc)::value, decltype(a)::value, I>, dim3(g.x, g.y, 2), dim3(KV4_THREADS), 0,
               (hipStream_t)stream, cache, out, (const I*)slots, (long)tokens, (int)heads, kv4_shift(page), (long)(pages * page), g.per, g.hb);
   });
   return kv4_status("hx_kv4_read");

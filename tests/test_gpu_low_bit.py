@@ -203,6 +203,25 @@ def test_kv4_write_the_last_token_of_a_slot_stays():
         assert torch.equal(r.cpu()[at], ref.decode(*ref.encode(x.float()))[src].float())
 
 
+@pytest.mark.parametrize("heads,tokens", [(12, 5000), (2, 70000), (5, 4100)])
+def test_kv4_write_many_heads_and_many_tokens(heads, tokens):
+    """several heads in one go with some left over, tokens beyond one launch, slots that repeat within and across launches"""
+    g = torch.Generator().manual_seed(heads)
+    k, v = (torch.randn(tokens, heads, 64, generator=g).to(HF) for _ in range(2))
+    n = tokens - tokens // 8
+    slots = torch.cat([torch.randperm(n, generator=g), torch.randperm(n, generator=g)])[:tokens].to(torch.int32)
+    slots[::97] = 5                                         # one slot again and again, in every group of tokens
+    cache = hx.kv4_cache(-(-n // 32), 32, heads, 64)
+    for t in cache:
+        t.zero_()
+    hx.kv4_write(cache, k.to(DEV), v.to(DEV), slots.to(DEV))
+    rk, rv = hx.kv4_read(cache, torch.arange(n, device=DEV, dtype=torch.int32), F32)
+    last = torch.full((n,), -1, dtype=torch.long).scatter_reduce_(0, slots.long(), torch.arange(tokens), "amax")
+    for r, x in ((rk, k), (rv, v)):
+        want = ref.decode(*ref.encode(x.float())).float()[last.clamp(min=0)] * (last >= 0)[:, None, None]
+        assert torch.equal(r.cpu(), want)
+
+
 def test_kv4_offsets_beyond_32_bits():
     """a cache of more than 4 GB of codes: its last page is written, read back and attended to"""
     heads, d, page = 8, 128, 64
