@@ -34,7 +34,7 @@ __global__ __launch_bounds__(KR_WAVES * 64, 2) void hx_kv4_attention_rows(KaArgs
   constexpr size_t LDS = sizeof(KrLds<D>) > sizeof(KaFewLds<D, KR_WAVES>) ? sizeof(KrLds<D>) : sizeof(KaFewLds<D, KR_WAVES>);
   __shared__ __attribute__((aligned(16))) uint8_t raw[LDS];
   KaSeq q;
-  if (!ka_sequence(a, q)) return;
+  if (!ka_sequence<true>(a, q)) return;
   if (q.rows <= 16) {  // (uniform)
     if (q.block0 == 0) ka_few<D, DT, NQ, DT == HX_F32 ? 3 : 2, 1, KR_WAVES, 2>(a, q, *(KaFewLds<D, KR_WAVES>*)raw);
     return;

@@ -278,6 +278,18 @@ def test_kv4_attention(dtype, dim, page, kv_heads, group, lens, news):
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("lens,news", [
+    ([(37 * i) % 61 for i in range(200)], None), ([20] * 300, None), ([17 * (i % 2) for i in range(129)], None),
+    ([3 + (11 * i) % 90 for i in range(131)], [1 + (7 * i) % 3 for i in range(131)]), ([500] + [5] * 139, None)])
+def test_kv4_attention_of_many_sequences(lens, news):
+    """more sequences than a wave has lanes, which run in the order of their lengths: different, equal, alternating ones"""
+    q, cache, table, n, start = lb.attention_case(BF, 64, 16, 8, 2, lens, news, seed=1)
+    qd, td, nd, sd = _dev(q, table, n, start)
+    cd = hx.Kv4Cache(*_dev(*cache))
+    out = hx.kv4_attention(qd, cd, td, nd, query_start=sd, max_query_len=max(news) if news else 1)
+    lb.check_attention(out, qd, cd, td, nd, sd)
+
+
 @pytest.mark.parametrize("dtype,many", [(BF, False), (HF, False), (BF, True), (HF, True)])
 def test_kv4_attention_masks(dtype, many):
     """many: 64 key/value heads with 16 query heads each, 112 rows, 512 workgroups of 128 (the kernel for pieces of prompts)"""
