@@ -92,6 +92,24 @@ def test_int8_gemm(m, n, k, bias, out, layout):
     assert torch.equal(got, hx.int8_gemm(xd, yd, sad.flatten(), sbd.flatten(), bias=bd, out_dtype=out))
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 40, 16), (16, 300, 1040), (30, 64, 9008), (33, 300, 1040), (64, 128, 8208), (200, 515, 48), (300, 260, 4112),
+                                   (2304, 2048, 144), (2304, 2060, 2064)])
+def test_int8_gemm_nothing_behind_k_counts(m, n, k):
+    """k a multiple of 16 but not of 128, read in place: what stands behind k in longer rows does not matter, on either side,
+    with the other one read in place too or copied"""
+    x, y, sa, sb, _ = lb.gemm_inputs(m, n, k, m + k, None, "col")
+    xd, yd, sad, sbd = _dev(x, y, sa, sb)
+    want = ((x.to(DEV).double() @ y.to(DEV).double()).float() * sad.view(-1, 1)) * sbd.view(1, -1)
+    wide = torch.full((m, k + 112), 127, dtype=torch.int8, device=DEV)
+    tall = torch.full((n, k + 112), -127, dtype=torch.int8, device=DEV)
+    wide[:, :k], tall[:, :k] = xd, yd.t()
+    odd_a, odd_b = torch.empty(m * k + 1, dtype=torch.int8, device=DEV)[1:].view(m, k), yd.contiguous()
+    odd_a.copy_(xd)
+    for a in (xd, wide[:, :k], odd_a):
+        for b in (yd, tall[:, :k].t(), odd_b):
+            assert torch.equal(hx.int8_gemm(a, b, sad, sbd, out_dtype=F32), want)
+
+
 def test_int8_gemm_strides_and_empty():
     x, y, sa, sb, _ = lb.gemm_inputs(70, 90, 256, 3)
     want = hx.int8_gemm(*_dev(x, y, sa, sb), out_dtype=F32)
