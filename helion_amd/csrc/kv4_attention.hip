@@ -25,6 +25,7 @@
 
 #define KA_M0 (-3e38f)  // the reference point of a row that has seen no key
 #define KA_PIECE 1024  // keys of a split at least
+#define KA_GRID (1l << 22)  // workgroups of a launch at most (2^32 work-items are too many for one)
 #define KA_STEP 8.f     // it moves only when a score lies 2^8 above it: p stays below 256, and few tiles rescale O
 
 int kv4_check_cache(const char* who, const void* kc, const void* ks, const void* vc, const void* vs, int64_t pages, int64_t page,
@@ -519,45 +520,47 @@ __global__ __launch_bounds__(256) void hx_kv4_attention_join(KaArgs a) {
   typedef typename KaT<DT>::T T;
   constexpr int E = D / 64;
   __shared__ float part[4][D];
-  const int row = blockIdx.x;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int t = (unsigned)row / (unsigned)a.heads;
-  if (a.query_start && (t < a.query_start[0] || t >= a.query_start[a.batch])) return;  // behind the last sequence
-  const float* ml = a.part_ml + (long)row * a.splits * 2;
-  const bool there = lane < a.splits;
-  float l = there ? ml[2 * lane + 1] : 0.f;
-  const float m = there ? ml[2 * lane] : KA_M0;
-  float top = m;
+  for (long row = blockIdx.x; row < (long)a.tokens * a.heads; row += gridDim.x) {
+    const int t = (unsigned)row / (unsigned)a.heads;  // (row < 2^31)
+    if (a.query_start && (t < a.query_start[0] || t >= a.query_start[a.batch])) continue;  // behind the last sequence
+    const float* ml = a.part_ml + row * a.splits * 2;
+    const bool there = lane < a.splits;
+    float l = there ? ml[2 * lane + 1] : 0.f;
+    const float m = there ? ml[2 * lane] : KA_M0;
+    float top = m;
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-  const float f = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - top);  // (a split without keys has written nothing else)
-  float sum = l * f;
+    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+    const float f = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - top);  // (a split without keys has written nothing else)
+    float sum = l * f;
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
-  float acc[E];
+    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
+    float acc[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  const float* o = a.part_o + (long)row * a.splits * D + lane * E;
-  for (int s0 = w; s0 < a.splits; s0 += 16) {
-    float v[4][E];
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    const float* o = a.part_o + row * a.splits * D + lane * E;
+    for (int s0 = w; s0 < a.splits; s0 += 16) {
+      float v[4][E];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[i][e] = o[(long)min(s0 + 4 * i, a.splits - 1) * D + e];
+        for (int e = 0; e < E; ++e) v[i][e] = o[(long)min(s0 + 4 * i, a.splits - 1) * D + e];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int s = s0 + 4 * i;
-      const float fs = __shfl(f, s & 63);
+      for (int i = 0; i < 4; ++i) {
+        const int s = s0 + 4 * i;
+        const float fs = __shfl(f, s & 63);
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (s < a.splits && fs != 0.f) acc[e] += v[i][e] * fs;
+        for (int e = 0; e < E; ++e)
+          if (s < a.splits && fs != 0.f) acc[e] += v[i][e] * fs;
+      }
     }
-  }
 #pragma unroll
-  for (int e = 0; e < E; ++e) part[w][lane * E + e] = acc[e];
-  __syncthreads();
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  for (int d = threadIdx.x; d < D; d += 256) ((T*)a.out)[(long)row * D + d] = (T)((part[0][d] + part[1][d] + part[2][d] + part[3][d]) * inv);
+    for (int e = 0; e < E; ++e) part[w][lane * E + e] = acc[e];
+    __syncthreads();
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    for (int d = threadIdx.x; d < D; d += 256) ((T*)a.out)[row * D + d] = (T)((part[0][d] + part[1][d] + part[2][d] + part[3][d]) * inv);
+    __syncthreads();
+  }
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
@@ -586,7 +589,7 @@ static KaPlan ka_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D,
   int64_t blocks = (rows + per - 1) / per;
   if (blocks < 1) blocks = 1;
   if (blocks > 65536) blocks = 65536;
-  while (blocks > 1 && batch * kv_heads * blocks > (1l << 30)) blocks /= 2;
+  while (blocks > 1 && kv_heads * blocks > KA_GRID) blocks /= 2;
   p.blocks = (int)blocks;
   // Keys are split, into pieces of at least 1024, until there are sixteen workgroups per compute unit (sequences differ in
   // length, and what ends last counts) or two of the larger ones; a sequence shorter than the table's width uses fewer.
@@ -630,7 +633,7 @@ extern "C" size_t hx_kv4_attention_workspace_bytes(int64_t tokens, int64_t batch
 
 template <int D, int DT>
 static void ka_launch(const KaArgs& a, const KaPlan& p, hipStream_t s) {
-  const dim3 grid((unsigned)((int64_t)a.kv_heads * a.batch * p.splits * p.blocks)), block(p.nw * 64);
+  const dim3 grid((unsigned)((int64_t)a.kv_heads * a.batch * p.splits * p.blocks)), block(p.nw * 64);  // (at most KA_GRID)
   constexpr int NQ = DT == HX_BF16 ? 1 : DT == HX_F16 ? 2 : 3, NP = DT == HX_F32 ? 3 : 2;
   if (p.many) {
     if constexpr (D <= 128 && DT != HX_F32) hx_launch(hx_kv4_attention_rows<D, DT, NQ, DT == HX_BF16 ? 1 : NP>, grid, dim3(KR_WAVES * 64), 0, s, a);
@@ -639,7 +642,7 @@ static void ka_launch(const KaArgs& a, const KaPlan& p, hipStream_t s) {
   } else if constexpr (D <= 128 && DT != HX_F32) {
     hx_launch(hx_kv4_attention_kernel<D, DT, NQ, DT == HX_BF16 ? 1 : NP, 2, 4, 2>, grid, block, 0, s, a);
   }
-  if (p.splits > 1) hx_launch(hx_kv4_attention_join<D, DT>, dim3((unsigned)((long)a.tokens * a.heads)), dim3(256), 0, s, a);
+  if (p.splits > 1) hx_launch(hx_kv4_attention_join<D, DT>, dim3((unsigned)min((long)a.tokens * a.heads, KA_GRID)), dim3(256), 0, s, a);
 }
 
 extern "C" int hx_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_codes, const void* k_scales,
@@ -698,9 +701,21 @@ extern "C" int hx_kv4_attention(const void* q, int64_t q_token_stride, int64_t q
     else if (dtype == HX_BF16) ka_launch<DC, HX_BF16>(a, p, (hipStream_t)stream);
     else ka_launch<DC, HX_F32>(a, p, (hipStream_t)stream);
   };
-  if (D == 64) go(std::integral_constant<int, 64>{});
-  else if (D == 128) go(std::integral_constant<int, 128>{});
-  else go(std::integral_constant<int, 256>{});
+  // as many sequences in a launch as it has room for (so many that their keys are not split)
+  const int64_t room = KA_GRID / (kv_heads * p.blocks * p.splits), es = dtype == HX_F32 ? 4 : 2;
+  for (int64_t b = 0; b < batch; b += room) {
+    a.batch = (int)(batch - b < room ? batch - b : room);
+    a.table = block_table + b * table_stride, a.seq_lens = seq_lens + b;
+    if (query_start) {
+      a.query_start = query_start + b;
+    } else {
+      a.q = (const char*)q + b * q_token_stride * es, a.out = (char*)out + b * heads * D * es;
+      a.tokens = a.batch;
+    }
+    if (D == 64) go(std::integral_constant<int, 64>{});
+    else if (D == 128) go(std::integral_constant<int, 128>{});
+    else go(std::integral_constant<int, 256>{});
+  }
   const hipError_t e = hx_launch_status();
   if (e != hipSuccess) {
     hx_set_error("%s: launch failed: %s", who, hipGetErrorString(e));

@@ -365,12 +365,19 @@ extern "C" int hx_kv4_read(const void* k_codes, const void* k_scales, const void
     hx_set_error("hx_kv4_read: k and v must be 16-byte aligned");
     return HX_ERR_UNSUPPORTED;
   }
-  Kv4Ptrs cache = {{(void*)k_codes, (void*)v_codes}, {(void*)k_scales, (void*)v_scales}}, out = {{k, v}, {nullptr, nullptr}};
-  const Kv4Grid g = kv4_grid(tokens, heads, D);
-  kv4_pick(dtype, D, g.hb, slots_are_int64, [&](auto dtc, auto dc, auto a, auto i) {
-    typedef decltype(i) I;
-    hx_launch(hx_kv4_read_kernel<decltype(dtc)::value, decltype(dc)::value, decltype(a)::value, I>, dim3(g.x, g.y, 2), dim3(KV4_THREADS), 0,
-              (hipStream_t)stream, cache, out, (const I*)slots, (long)tokens, (int)heads, kv4_shift(page), (long)(pages * page), g.per, g.hb);
-  });
+  Kv4Ptrs cache = {{(void*)k_codes, (void*)v_codes}, {(void*)k_scales, (void*)v_scales}};
+  const int64_t es = dtype == HX_F32 ? 4 : 2, most = 1l << 20;  // (a launch has room for fewer than 2^32 work-items)
+  for (int64_t first = 0; first < tokens; first += most) {
+    const int64_t n = tokens - first < most ? tokens - first : most;
+    const Kv4Grid g = kv4_grid(n, heads, D);
+    const int64_t at = first * heads * D * es;
+    Kv4Ptrs out = {{(char*)k + at, (char*)v + at}, {nullptr, nullptr}};
+    kv4_pick(dtype, D, g.hb, slots_are_int64, [&](auto dtc, auto dc, auto a, auto i) {
+      typedef decltype(i) I;
+      hx_launch(hx_kv4_read_kernel<decltype(dtc)::value, decltype(dc)::value, decltype(a)::value, I>, dim3(g.x, g.y, 2), dim3(KV4_THREADS),
+                0, (hipStream_t)stream, cache, out, (const I*)slots + first, (long)n, (int)heads, kv4_shift(page), (long)(pages * page), g.per,
+                g.hb);
+    });
+  }
   return kv4_status("hx_kv4_read");
 }

@@ -166,8 +166,13 @@ static void nq_launch(const void* x, long xs, const void* res, long rs, const vo
   const bool few = rows <= 2 * hx_cu_count();
   auto go = [&](auto kernel, int tpr) {
     const int rpw = tpr < 256 ? 256 / tpr : 1;
-    hx_launch(kernel, dim3((unsigned)((rows + rpw - 1) / rpw)), dim3(tpr < 256 ? 256 : tpr), 0, s, (const T*)x, xs, (const T*)res, rs,
-              (const T*)w, eps, (T*)h, (signed char*)q, scale, rows, width);
+    const long most = (1l << 31) / tpr;  // (a launch has room for fewer than 2^32 work-items)
+    for (long at = 0; at < rows; at += most) {
+      const long n = rows - at < most ? rows - at : most;
+      hx_launch(kernel, dim3((unsigned)((n + rpw - 1) / rpw)), dim3(tpr < 256 ? 256 : tpr), 0, s, (const T*)x + at * xs, xs,
+                RES ? (const T*)res + at * rs : nullptr, rs, (const T*)w, eps, RES ? (T*)h + at * width : nullptr,
+                (signed char*)q + at * width, scale + at, n, width);
+    }
   };
   if (width <= 512) go(hx_norm_int8_kernel<DT, 64, 1, NORM, RES, NT>, 64);
   else if (width <= 1024) go(hx_norm_int8_kernel<DT, 64, 2, NORM, RES, NT>, 64);

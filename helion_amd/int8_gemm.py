@@ -1,6 +1,6 @@
 """Linear layers in 8-bit integers: the product with a scale for each token and each output channel, and the two
 producers of its operands, quantisation by rows and the root-mean-square norm that ends in it.  (The per-tensor e4m3
-counterparts are ``fp8_gemm_scaled`` and ``fp8_quantize_per_tensor``.)"""
+counterparts are ``fp8_gemm_scaled`` and ``fp8_quantize_per_tensor``.)  For inference: no result carries a gradient."""
 from __future__ import annotations
 
 import torch
@@ -13,8 +13,7 @@ def int8_gemm(x: torch.Tensor, y: torch.Tensor, scale_a: torch.Tensor, scale_b: 
     """``out[m, n] = cast(sum_k x[m, k] * y[k, n] * scale_a[m] * scale_b[n] + bias[n])``.
 
     x: [m, k] int8, y: [k, n] int8 with any strides; ``w.t()`` of a contiguous [n, k] weight with ``k % 16 == 0`` is the fast
-    layout (read in place, and x too where ``k % 128 == 0``; other operands are copied once into a workspace).  The sum is
-    exact (``k <= 131071``); scales (float32, m and n elements in any shape) and bias (n elements of float16, bfloat16 or
+    layout (both operands are read in place; others are copied into a workspace first).  The sum is exact (``k <= 131071``); scales (float32, m and n elements in any shape) and bias (n elements of float16, bfloat16 or
     float32) are applied in fp32.  out_dtype: float16, bfloat16 or float32."""
     return int8_gemm_call(x, y, scale_a, scale_b, bias, out_dtype)
 
@@ -33,7 +32,7 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
     """Root-mean-square norm over the last dimension with 8-bit output: ``(q, scale)`` of
     ``h * rsqrt(mean(h^2) + eps) * weight`` as in :func:`int8_quantize_per_token`, with ``h = x``; or, with a residual of x's
     shape, ``(q, scale, h)`` with ``h = x + residual`` rounded to x's dtype: the new residual, of whose rounded values the
-    norm is taken.  weight: [width] of x's dtype.  One launch; everything behind h is fp32."""
+    norm is taken.  weight: [width] of x's dtype.  Everything behind h is fp32."""
     if residual is None:
         return rms_norm_int8_call(x, weight, eps)
     return add_rms_norm_int8_call(x, residual, weight, eps)

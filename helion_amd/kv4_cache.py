@@ -3,7 +3,7 @@
 The format is MXFP4: e2m1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) with a power-of-two scale for each 32
 consecutive elements of a head, 4.25 bits an element.  The rounding is to the nearest value, ties to the even code; what a
 block's exponent ``floor(log2 max|x|) - 2`` leaves above 6 becomes 6.  The layout of the four tensors is part of the C
-interface (include/hx_kernels.h)."""
+interface (include/hx_kernels.h).  For inference: no result carries a gradient."""
 from __future__ import annotations
 
 from typing import NamedTuple
@@ -45,7 +45,7 @@ def kv4_write(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Te
     """Quantise k and v, [tokens, heads, head_dim] float16, bfloat16 or float32, into the cache: token t goes to
     ``slots[t] = page * page_size + place`` (int32 or int64).  k and v may be slices of one projection's output (any token and
     head strides).  A slot outside the cache (-1 for a padded token) writes nothing; of several tokens with one slot the last
-    one stays.  One launch."""
+    one stays.  One launch for every 32768 tokens."""
     kv4_write_call(*cache, k, v, slots)
 
 

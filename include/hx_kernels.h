@@ -284,7 +284,7 @@ int hx_attention_path(int64_t BH, int64_t M, int64_t N, int64_t D, int dtype, co
  * A row whose y holds a NaN or an infinity gets that as its scale and zeros as its integers (0 * scale is NaN).
  * x, residual: rows x width of `dtype` (HX_F16 / HX_BF16 / HX_F32), elements of a row contiguous, row strides in elements;
  * weight [width] of the same dtype; h_out (with a residual), q and scale are contiguous.  1 <= width <= 65536, any rows,
- * pointers aligned to their elements.  One launch, no workspace. */
+ * pointers aligned to their elements.  No workspace. */
 int hx_rms_norm_int8(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight, float eps,
                      void* h_out, void* q, float* scale, int64_t rows, int64_t width, int dtype, void* stream);
 int hx_int8_quantize_per_token(const void* x, int64_t x_stride, void* q, float* scale, int64_t rows, int64_t width, int dtype,
@@ -296,8 +296,8 @@ int hx_int8_quantize_per_token(const void* x, int64_t x_stride, void* q, float* 
  * contiguous bytes, row stride lda >= K; b addressed as b[k*ldb_k + n*ldb_n], strides >= 1; bias [N] of bias_dtype or NULL;
  * out_dtype HX_F16 / HX_BF16 / HX_F32, row stride ldc.  Any M, N and K >= 1 below 4 GB per operand.  b with ldb_k == 1
  * (the [N][K] weight of a linear layer), K % 16 == 0 and 16-byte aligned rows is read in place, everything else is copied
- * into the workspace first; K % 128 != 0 copies a.  workspace: hx_int8_gemm_workspace_bytes(...) bytes (copies, and the
- * integer sums of a split K), 256-byte aligned. */
+ * into the workspace first, and so is an a whose rows are not 16-byte aligned or K % 16 != 0.  workspace:
+ * hx_int8_gemm_workspace_bytes(...) bytes (copies, and the integer sums of a split K), 256-byte aligned. */
 int hx_int8_gemm(const void* a, const void* b, void* c, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb_k, int64_t ldb_n,
                  int64_t ldc, const float* scale_a, const float* scale_b, const void* bias, int bias_dtype, int out_dtype,
                  void* workspace, size_t workspace_bytes, void* stream);
@@ -315,7 +315,7 @@ size_t hx_int8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t lda
  *
  * hx_kv4_write: k, v [tokens][heads][D] of `dtype` (HX_F16 / HX_BF16 / HX_F32), elements of a head contiguous, token and head
  * strides in elements; slots: tokens int32 or int64 values.  A token whose slot lies outside 0 .. pages*page-1 (-1 for
- * padding) is not written; of several tokens with the same slot the last one is.  One launch, no workspace.
+ * padding) is not written; of several tokens with the same slot the last one is.  One launch per 32768 tokens, no workspace.
  * hx_kv4_read: the values at the slots into k, v [tokens][heads][D], contiguous and 16-byte aligned, rounded to `dtype`;
  * zeros for a slot outside. */
 int hx_kv4_write(const void* k, const void* v, void* k_codes, void* k_scales, void* v_codes, void* v_scales, const void* slots,

@@ -485,3 +485,45 @@ def test_traced_entry_points():
     want = step([t.clone() for t in cd])
     got = torch.compile(step, backend="eager", fullgraph=True)([t.clone() for t in cd])
     assert all(torch.equal(i, j) for i, j in zip(got, want))
+
+
+# ---------------------------------------------------------------------------------------------- more than one launch holds
+def test_more_rows_than_a_launch_holds():
+    """70 million rows, more work-items than one launch may have: every row stands for itself, so a piece on its own agrees"""
+    rows = 70_000_000
+    x = torch.randn(rows, 8, device=DEV, dtype=HF, generator=torch.Generator(DEV).manual_seed(0))
+    w = torch.linspace(0.5, 2.0, 8, device=DEV).to(HF)
+    q, s = hx.int8_quantize_per_token(x)
+    nq, ns, h = hx.rms_norm_int8(x, w, residual=x)
+    assert torch.equal(h, x + x)
+    for at in (0, 2**25 - 3, 2**26 - 3, rows - 6):
+        piece = slice(at, at + 6)
+        for got, want in zip((q, s, nq, ns), (*hx.int8_quantize_per_token(x[piece]), *hx.rms_norm_int8(x[piece], w, residual=x[piece])[:2])):
+            assert torch.equal(got[piece], want)
+
+
+def test_more_tokens_read_than_a_launch_holds():
+    cache = hx.kv4_cache(2, 64, 1, 64)
+    k = torch.randn(128, 1, 64, device=DEV, dtype=HF)
+    hx.kv4_write(cache, k, -k, torch.arange(128, device=DEV))
+    slots = (torch.arange(2**20 + 77, device=DEV) * 7) % 131 - 1
+    rk, rv = hx.kv4_read(cache, slots, dtype=HF)
+    one = hx.kv4_read(cache, torch.arange(-1, 130, device=DEV), dtype=HF)
+    assert torch.equal(rk, one[0][slots + 1]) and torch.equal(rv, one[1][slots + 1])
+
+
+@pytest.mark.parametrize("starts", [False, True])
+def test_more_sequences_than_a_launch_holds(starts):
+    batch, heads = 2**20 + 3, 8
+    cache = hx.kv4_cache(1, 16, heads, 64)
+    k = torch.randn(16, heads, 64, device=DEV, dtype=HF)
+    hx.kv4_write(cache, k, k.flip(0), torch.arange(16, device=DEV))
+    q = torch.randn(batch, heads, 64, device=DEV, dtype=HF)
+    table = torch.zeros(batch, 1, dtype=torch.int32, device=DEV)
+    lens = (torch.arange(batch, device=DEV) % 17).int()
+    start = torch.arange(batch + 1, device=DEV).int() if starts else None
+    out = hx.kv4_attention(q, cache, table, lens, query_start=start, max_query_len=1)
+    for at in (0, 2**19 - 20, 2**20 - 20, batch - 40):
+        piece = slice(at, at + 40)
+        want = hx.kv4_attention(q[piece], cache, table[piece], lens[piece])
+        assert torch.equal(out[piece], want) and not want[lens[piece] > 0].eq(0).all()

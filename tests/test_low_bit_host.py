@@ -43,7 +43,8 @@ def test_int8_gemm_refusals_and_workspace():
     assert gemm(bk=4, bn=1) == -3 and b"workspace" in lib.hx_last_error()           # another stride order: copied
     need = lambda m, n, k, lda, bk, bn, a=A, b=A: lib.hx_int8_gemm_workspace_bytes(m, n, k, lda, bk, bn, a, b)
     assert need(300, 300, 256, 256, 1, 256) == 0
-    assert need(300, 300, 272, 272, 1, 272) == 300 * 384 + (-300 * 384) % 256        # a copied, b read in place
+    assert need(300, 300, 272, 272, 1, 272) == 0                                     # both read in place and behind k
+    assert need(300, 300, 272, 272, 1, 272, A + 1) == 300 * 384 + (-300 * 384) % 256 # a copied, b read in place
     assert need(300, 300, 256, 256, 1, 256, A + 1) == 300 * 256 and need(300, 300, 256, 256, 1, 256, A, A + 8) == 300 * 256
     assert need(300, 300, 100, 100, 1, 100) == 2 * 300 * 128 + 2 * (-300 * 128 % 256)
     assert need(0, 4, 4, 4, 1, 4) == 0 and need(4, 4, 200000, 200000, 1, 200000) == 0
