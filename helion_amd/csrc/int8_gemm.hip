@@ -576,15 +576,6 @@ struct I8Plan {
   size_t a_off, b_off, part_off, bytes;
 };
 
-// Rows of the tile: 64 or 128 (of 128 columns), or 256 (of 256).  All run one workgroup per compute unit, so a launch takes
-// ceil(tiles / 256) rounds of nk steps plus what a tile costs outside its loop, and the cheaper estimate wins.
-static int i8_rows(int64_t M, int64_t N, int64_t nk) {
-  if (M <= 64) return 64;
-  const int64_t cus = hx_cu_count();
-  auto rounds = [&](int64_t t) { return (((M + t - 1) / t) * ((N + t - 1) / t) + cus - 1) / cus; };
-  return M > 128 && rounds(256) * (150 * nk + 600) <= rounds(128) * (45 * nk + 460) ? 256 : 128;
-}
-
 static void i8_offsets(I8Plan& p, int64_t M, int64_t N) {
   size_t at = 0;
   auto take = [&](bool want, int64_t bytes) {
@@ -621,18 +612,25 @@ static I8Plan i8_plan(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb_
   p.tail = K % I8_BK != 0 && !(p.copy_a && p.copy_b);
   p.ns = -1;
   if (M <= 32) return i8_plan_skinny(p, M, N, K);
-  p.bm = i8_rows(M, N, p.ka / I8_BK);
-  p.bn = p.bm == 256 ? 256 : 128;
-  const int64_t tiles = ((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn), nk = p.ka / I8_BK;
-  // Few tiles and a long K: the k-tiles of a tile are divided among workgroups, eight at least for each, and the partial
-  // sums stay below 32 MB.
-  int64_t s = p.bm == 256 ? 1 : hx_cu_count() / tiles;
-  if (s > nk / 8) s = nk / 8;
-  while (s > 1 && s * M * N * 4 > (32LL << 20)) --s;
-  p.splits = 1, p.kt_per_split = 0;
-  if (s > 1) {
-    p.kt_per_split = (int)((nk + s - 1) / s);
-    p.splits = (int)((nk + p.kt_per_split - 1) / p.kt_per_split);
+  // Rows of the tile, 64 or 128 (of 128 columns) or 256 (of 256), and workgroups that share the k-tiles of one: what a
+  // launch takes in units of 10 ns, from rounds of one workgroup per compute unit, a k-tile's time and what surrounds the
+  // loop, and for a split the partial sums' way through memory and the second launch.  At least eight k-tiles each, partial
+  // sums below 32 MB.  Measured with 64, 128, 256 rows: 512 x 4096 x 4096 15.4, 20 (23.5 split in two), 44 us; 128 x 8192 x
+  // 8192 21.2 (in two), 25.0 (in four), 76; 777 x 4096 x 4096 28.3, 20.4, 45; 1024 x 8192 x 8192 98.6, 70.8, 87.5;
+  // 8192 x 8192 x 8192 128 and 256 rows: 721 and 411.
+  const int64_t nk = p.ka / I8_BK, cus = hx_cu_count();
+  static const struct { int bm, bn, step, around; } tile[3] = {{64, 128, 33, 360}, {128, 128, 47, 530}, {256, 256, 150, 600}};
+  int64_t least = INT64_MAX;
+  for (const auto& t : tile) {
+    const int64_t tiles = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
+    if (t.bm == 256 && M <= 128) continue;
+    for (int64_t s = 1; s == 1 || (t.bm != 256 && s * tiles <= cus && 8 * s <= nk && s * M * N * 4 <= (32LL << 20)); ++s) {
+      const int64_t per = (nk + s - 1) / s, n = (nk + per - 1) / per;
+      const int64_t cost = (tiles * n + cus - 1) / cus * (t.step * per + t.around) + (n > 1 ? 300 + n * M * N * 4 / 20000 : 0);
+      if (cost >= least) continue;
+      least = cost;
+      p.bm = t.bm, p.bn = t.bn, p.splits = (int)n, p.kt_per_split = n > 1 ? (int)per : 0;
+    }
   }
   i8_offsets(p, M, N);
   return p;
