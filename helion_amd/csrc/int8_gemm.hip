@@ -37,6 +37,9 @@ __device__ __forceinline__ float i8_bias(const void* bias, int dt, long n) {
 // kq = 0, 3, 1, 2 (the order in which the 16-byte reads of a wave meet no bank twice).
 // split-K (kt_per_split): workgroup row blockIdx.y adds up its k-tiles into its own slab of 32-bit integers.
 // KT: K is not a multiple of 128 and A or B is read on behind it.
+// For batches between a decode step and a prompt: 777 x 4096 x 4096 (one round of 224 tiles of 128) 20.6 us, 512 x 4096 x
+// 4096 (256 of 64) 15.5.  A k-tile takes 0.47 and 0.33 us, of which its MFMAs are 0.21 and 0.11: with one workgroup per
+// compute unit the rest is the barrier, the LDS and the landing of the next k-tile.
 // ------------------------------------------------------------------------------------------
 template <int OUT, int BM, bool KT, bool SPLIT>
 __global__ __launch_bounds__(256) void hx_int8_gemm_tile(I8Args p) {
@@ -215,6 +218,8 @@ __global__ __launch_bounds__(256) void hx_int8_gemm_tile(I8Args p) {
 // blocks): under the first one the DMA of tile kt+2 goes out into this tile's own stage, whose fragments are all in
 // registers; between the halves "tile kt+1 has landed" is awaited; under the second the fragments of tile kt+1 replace
 // those that have had their last MFMA.  Rows past M or N re-read the last one and are not stored.
+// Bound by the matrix pipes and power: 8192 x 8192 x 8192 404 to 420 us, 2.6 to 2.7 POP/s, with an MFMA in 68 % of the busy
+// cycles (tiles of 128 x 128: 721 us, twice the LDS traffic per MFMA).
 // ------------------------------------------------------------------------------------------
 template <int OUT, bool KT>
 __global__ __launch_bounds__(256) void hx_int8_gemm_tile256(I8Args p) {
@@ -400,6 +405,8 @@ __global__ __launch_bounds__(256) void hx_int8_gemm_tile256(I8Args p) {
 // NS > 0: every wave has NS steps and the loads in flight can be counted; NS = 0: any number up to eight, and a K that is
 // not a multiple of 128 (rows are read on, clamped to the end of the matrix, and A becomes zero there).
 // split (gridDim.y > 1): workgroup row y adds up its steps into its own slab of 32-bit integers.
+// Bound by memory: 16 x 28672 x 8192 37.0 us, 6.3 TB/s (through the LDS tiles above 50.6), 32 rows 43.0 (48.4), 1 x 4096 x
+// 4096 4.8 (10.7).
 // ------------------------------------------------------------------------------------------
 #define I8S_WAVES 8
 #define I8S_STEPS 8

@@ -176,6 +176,8 @@ __device__ __forceinline__ void ka_queries(const KaArgs& a, const KaSeq& q, int 
 }
 
 // Rows in blocks of 16 RB; the waves of the workgroup take key tiles in turn and join what they have at the end.
+// What bounds it: the vector pipes (codes to bf16, softmax) in 60 to 73 % of the busy cycles, next to memory.  32 sequences of
+// up to 32768 keys, 8 heads of 128, 8 query heads each: 117 us, 5.0 TB/s; 64 sequences x 32 heads of 64, up to 2048 keys: 37.
 template <int D, int NW>
 struct KaFewLds {
   float joint[NW][16][D + 4];  // (padded rows)
