@@ -5,8 +5,10 @@
 //
 // Precision: an e2m1 value times a power of two is a bf16 number, so keys and values enter the matrix instructions
 // exactly.  The other operand of each product is a sum of bf16 terms: one for a bf16 query, two for fp16 (11 bits fit in
-// 16), three for fp32; p as two terms (2^-17 of it is lost) or three for fp32, or as one where a comment says so.  Products are
-// summed in fp32, as are the statistics.
+// 16), three for fp32; p as two terms (2^-17 of it is lost) or three for fp32, in every kernel, so that a row's precision
+// does not depend on the batch around it.  (One term for a bf16 result is faster, 322 instead of 438 us for 2048 new tokens
+// over 10240 keys, but then the weights' rounding adds to the result's: 1.4 times its error.)  Products are summed in fp32,
+// as are the statistics.
 //
 // Work: a workgroup takes RB blocks of 16 rows (a row = a new token of one query head) of one sequence and one key/value
 // head, so that all G heads share what is read and converted; its waves take key tiles of 32 tokens in turn, each with a
@@ -579,9 +581,10 @@ static KaPlan ka_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D,
   p.nw = 4;
   p.many = false;
   // 128 rows per workgroup with the conversion shared, or 32 with the keys divided among the waves: both run two workgroups
-  // per compute unit; for 128 keys the former takes 4.5 us in whole rounds (the workgroups end together), the latter 1.2 in
-  // as many rounds as it takes.  2048 tokens over 10240 keys 323 and 340 us, 8 x 512 over 2048 139 and 164; but 12 x 200
-  // over 4000 221 and 198, 2 x 512 over 4096 109 and 83.
+  // per compute unit; in units of time, the former takes 45 for as many keys as the latter takes 12 for, in whole rounds (its
+  // workgroups end together), the latter in as many rounds as it takes.  bf16, 32 heads of 128 on 8: 8 x 512 tokens over 2048
+  // keys 183 and 203 us, 4 x 1024 over 4096 345 and 361, 2048 over 10240 438 both; but 12 x 200 over 4000 280 and 243, 2 x 512
+  // over 4096 137 and 103.
   if (p.rb == 2 && rows > 64) {
     const int64_t slots = 2 * hx_cu_count(), pairs = batch * kv_heads;
     const int64_t many = (pairs * ((rows + KR_ROWS - 1) / KR_ROWS) + slots - 1) / slots * slots * 45, few = pairs * ((rows + 31) / 32) * 12;
@@ -638,11 +641,11 @@ static void ka_launch(const KaArgs& a, const KaPlan& p, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.kv_heads * a.batch * p.splits * p.blocks)), block(p.nw * 64);  // (at most KA_GRID)
   constexpr int NQ = DT == HX_BF16 ? 1 : DT == HX_F16 ? 2 : 3, NP = DT == HX_F32 ? 3 : 2;
   if (p.many) {
-    if constexpr (D <= 128 && DT != HX_F32) hx_launch(hx_kv4_attention_rows<D, DT, NQ, DT == HX_BF16 ? 1 : NP>, grid, dim3(KR_WAVES * 64), 0, s, a);
+    if constexpr (D <= 128 && DT != HX_F32) hx_launch(hx_kv4_attention_rows<D, DT, NQ, NP>, grid, dim3(KR_WAVES * 64), 0, s, a);
   } else if (p.rb == 1) {
     hx_launch(hx_kv4_attention_kernel<D, DT, NQ, NP, 1, 4, 2>, grid, block, 0, s, a);
   } else if constexpr (D <= 128 && DT != HX_F32) {
-    hx_launch(hx_kv4_attention_kernel<D, DT, NQ, DT == HX_BF16 ? 1 : NP, 2, 4, 2>, grid, block, 0, s, a);
+    hx_launch(hx_kv4_attention_kernel<D, DT, NQ, NP, 2, 4, 2>, grid, block, 0, s, a);
   }
   if (p.splits > 1) hx_launch(hx_kv4_attention_join<D, DT>, dim3((unsigned)min((long)a.tokens * a.heads, KA_GRID)), dim3(256), 0, s, a);
 }

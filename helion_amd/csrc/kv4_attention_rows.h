@@ -7,10 +7,11 @@
 // Every wave reads all fragments for its own two blocks of 16 rows; scores, statistics and outputs stay in its registers
 // and nothing is joined at the end.
 //
-// What bounds it (2048 new tokens of 32 heads over 10240 keys, bf16, head dim 128: 323 us, 0.96 PFLOP/s): for 32 keys a
-// wave's MFMAs take 544 cycles, its vector instructions (a quarter of them exponentials at a quarter of the rate) about
-// 500, its 16 KB of fragments a quarter of 500 cycles of the LDS; two waves per SIMD hide little more than half of that
-// behind each other.  Tried and slower: scores one half tile ahead in the wave (385), equal priorities (338).
+// What bounds it (2048 new tokens of 32 heads over 10240 keys, head dim 128: bf16 438 us, 0.71 PFLOP/s of the formula's
+// products; fp16 496): for 32 keys a wave's MFMAs take 832 cycles (16 for the scores, 32 for the two terms of the weights, 4 for
+// their sums, 16 cycles each), its vector instructions (a quarter of them exponentials at a quarter of the rate) about 650,
+// its 16 KB of fragments a quarter of 500 cycles of the LDS; two waves per SIMD hide little of that behind each other.
+// Tried and slower (with one term a weight, 323 us): scores one half tile ahead in the wave (385), equal priorities (338).
 //
 // A sequence with at most 16 rows (a single token in a mixed batch) is worked on as in ka_few instead.
 #define KR_WAVES 4
@@ -25,8 +26,6 @@ struct KrLds {
   uint8_t nan_at[2][4][64];  // the NaN values of each lane, one bit per token (where odd says so)
 };
 
-// weights as one bf16 term where the result is rounded to bf16 anyway: 2^-9 of a weight, at random, is what the rounding of
-// the result itself costs (measured: 1.35 times the error of exact weights)
 template <int D, int DT, int NQ, int NP>
 __global__ __launch_bounds__(KR_WAVES * 64, 2) void hx_kv4_attention_rows(KaArgs a) {
   typedef typename KaT<DT>::T T;
@@ -36,12 +35,12 @@ __global__ __launch_bounds__(KR_WAVES * 64, 2) void hx_kv4_attention_rows(KaArgs
   KaSeq q;
   if (!ka_sequence<true>(a, q)) return;
   if (q.rows <= 16) {  // (uniform)
-    if (q.block0 == 0) ka_few<D, DT, NQ, DT == HX_F32 ? 3 : 2, 1, KR_WAVES, 2>(a, q, *(KaFewLds<D, KR_WAVES>*)raw);
+    if (q.block0 == 0) ka_few<D, DT, NQ, NP, 1, KR_WAVES, 2>(a, q, *(KaFewLds<D, KR_WAVES>*)raw);
     return;
   }
   KrLds<D>& lds = *(KrLds<D>*)raw;
   // Two waves share a SIMD, and with equal rights they drift into the same phase and wait for the same pipe: one of them
-  // goes first wherever both can (2048 new tokens over 10240 keys 338 -> 323 us, head dim 64 74 -> 66).
+  // goes first wherever both can (with one term a weight, 2048 new tokens over 10240 keys 338 -> 323 us, head dim 64 74 -> 66).
   if (hx_wave_slot() & 1) __builtin_amdgcn_s_setprio(2);
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -63,7 +62,7 @@ __global__ __launch_bounds__(KR_WAVES * 64, 2) void hx_kv4_attention_rows(KaArgs
     ka_queries<D, DT, NQ, RB>(a, q, row0, qf, last);
     v4f o[RB][VJ];
     float mx[RB];
-    v4f l[RB];  // sums of the weights as multiplied: rows of ones times them, so that what is rounded off a weight is off both
+    v4f l[RB];  // sums of the weights as multiplied: rows of ones times them
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       mx[rb] = KA_M0;

@@ -1,6 +1,8 @@
 """Inputs and checks shared by the CPU and GPU tests of the low-bit serving operators."""
 from __future__ import annotations
 
+import math
+
 import torch
 
 from oracle import low_bit as ref
@@ -114,3 +116,17 @@ ATTENTION = [
     (BF, 128, 32, 1, 16, [90], [5]),                         # more than 16 rows
     (HF, 64, 16, 1, 3, [25], [25]),
 ]
+
+
+def cancelling_case(dtype, dim, page, kv_heads, group, lens, news):
+    """Values that cancel: the keys at even places have 1.5 times the weight of the others (as near as q's type allows) and
+    values of 1 against -1.5, so a result is near zero and what its weights lose by rounding stands alone."""
+    q, cache, table, n, start = attention_case(dtype, dim, page, kv_heads, group, lens, news)
+    pages = cache[0].shape[0]
+    k, v = torch.zeros(pages, kv_heads, page, dim), torch.ones(pages, kv_heads, page, dim)
+    k[:, :, 0::2, 0] = 1
+    v[:, :, 1::2] = -1.5
+    cache = (*ref.to_layout(*ref.encode(k), False), *ref.to_layout(*ref.encode(v), True))
+    q = torch.zeros_like(q)
+    q[..., 0] = (math.log(1.5) * dim**0.5 + 0.02 * torch.arange(q.shape[0] * q.shape[1]).view(q.shape[:2]).remainder(7)).to(dtype)
+    return q, cache, table, n, start

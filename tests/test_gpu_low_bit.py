@@ -527,3 +527,22 @@ def test_more_sequences_than_a_launch_holds(starts):
         piece = slice(at, at + 40)
         want = hx.kv4_attention(q[piece], cache, table[piece], lens[piece])
         assert torch.equal(out[piece], want) and not want[lens[piece] > 0].eq(0).all()
+
+
+# ---------------------------------------------------------------------------------------------- precision of the weights
+@pytest.mark.parametrize("dim,page,kv_heads,group,lens,news", [
+    (128, 16, 1, 8, [90, 33], [5, 4]), (64, 32, 2, 20, [700, 1], None), (128, 64, 8, 8, [300 + 9 * i for i in range(32)], [64] * 32),
+    (64, 16, 64, 16, [40, 33] * 4, [5, 7] * 4), (128, 32, 8, 4, [1000, 64] * 6, [100, 1] * 6),
+])
+@pytest.mark.parametrize("case", [lb.attention_case, lb.cancelling_case])
+def test_kv4_attention_weights_lose_nothing_to_a_batch(case, dim, page, kv_heads, group, lens, news):
+    """the weights are two bf16 terms whichever kernel a batch's rows lead to (32 rows a workgroup, or 128 where they fill the
+    chip): results near zero show what they lose"""
+    q, cache, table, n, start = _dev_case(case(BF, dim, page, kv_heads, group, lens, news))
+    out = hx.kv4_attention(q, cache, table, n, query_start=start, max_query_len=max(news) if news else 1)
+    lb.check_attention(out, q, cache, table, n, start, p_terms=2)
+
+
+def _dev_case(case):
+    q, cache, table, n, start = case
+    return (q.to(DEV), hx.Kv4Cache(*_dev(*cache)), *_dev(table, n, start))

@@ -242,3 +242,18 @@ def test_kv4_attention_no_pages():
     cache = _empty(0, 1, 16, 64)
     out = simops.kv4_attention(q, cache, torch.zeros(2, 1, dtype=torch.int32), torch.tensor([5, 0], dtype=torch.int32), fill=0xFF)
     assert (out == 0).all()
+
+
+# (dtype, dim, page, kv_heads, group, lens, new tokens, compute units): 32 rows a workgroup, and 128
+WEIGHTS = [(BF, 128, 16, 1, 8, [90, 33], [5, 4], 256), (BF, 64, 32, 1, 20, [70], None, 256), (BF, 128, 16, 1, 4, [90, 70], [33, 4], 1),
+           (BF, 64, 16, 1, 3, [129], [64], 1)]
+
+
+@pytest.mark.parametrize("dtype,dim,page,kv_heads,group,lens,news,cus", WEIGHTS)
+@pytest.mark.parametrize("case", [lb.attention_case, lb.cancelling_case])
+def test_kv4_attention_weights_lose_nothing_to_a_batch(case, dtype, dim, page, kv_heads, group, lens, news, cus):
+    """the weights are two bf16 terms whichever kernel a batch's rows lead to: results near zero show what they lose"""
+    q, cache, table, n, start = case(dtype, dim, page, kv_heads, group, lens, news)
+    with simlib.cus(cus):
+        out = simops.kv4_attention(q, cache, table, n, start)
+    lb.check_attention(out, q, cache, table, n, start, p_terms=2)
