@@ -3,13 +3,18 @@
 //   hx_int8_quantize_per_token y = x
 //   both: scale = max|y| / 127 (1 for a row of zeros),  q = round_to_nearest_even(y * 127 / max|y|)
 // so that q * scale ~ y: the (tensor, scale) pairs hx_int8_gemm reads.  h, the residual stream, is rounded to the
-// activations' type once and the norm is taken of the rounded values (they are what the next layer adds to); everything
-// from there to q stays in fp32.  A row with a NaN or an infinity in y gets that as its scale and zeros as its integers.
+// activations' type once and the norm is taken of the rounded values (they are what the next layer adds to).  A row with a NaN
+// or an infinity in y gets that as its scale and zeros as its integers.
+//
+// Precision: the root cancels in y / max|y|, so the integers need only the products h * weight, which fp32 holds exactly for
+// 16-bit types (for fp32 they are rounded once), and a quotient rounded in fp64: a value next to the middle between two
+// integers falls to the formula's side.  (All in fp32 some thirty of a million integers fell to the other.)  The mean of
+// the squares is summed in fp64, where no square of an fp32 number overflows, and the scale is rounded once.
 //
 // Bound by memory: x (and the residual) are read once, h, q and the scale written once.  A row lives in the registers of
 // the lanes that share it, so neither the mean nor the maximum costs a second read; the two reductions go through the
 // wave's shuffles and, where several waves share a row, four or sixteen floats of LDS.  8192 x 8192 bf16 with a residual:
-// 89 us, 470 MB at 5.3 TB/s; one row 4.1 us.
+// 86 us, 470 MB at 5.5 TB/s; one row 4.6 us.
 #include "hx_common.h"
 
 #include <type_traits>
@@ -60,42 +65,49 @@ __device__ __forceinline__ void nq_store(T* __restrict__ p, int left, const T (&
   }
 }
 
-// Sum / largest pattern over the TPR lanes that share a row (the whole workgroup, or one wave of four)
+// Sum and largest pattern over the TPR lanes that share a row (the whole workgroup, or one wave of four), together: the two
+// chains of shuffles run side by side and share a barrier.
 template <int TPR>
-__device__ __forceinline__ float nq_sum(float v, float* red) {
+struct NqLds {
+  double sum[TPR / 64];
+  unsigned top[2][TPR / 64];
+};
+template <int TPR, bool SUM>
+__device__ __forceinline__ void nq_join(double& sum, unsigned& top, NqLds<TPR>& lds, int turn) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
-  if (TPR == 64) return v;
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  for (int off = 32; off > 0; off >>= 1) {
+    if (SUM) {
+      const uint64_t u = __builtin_bit_cast(uint64_t, sum);
+      const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)u, off), hi = (uint32_t)__shfl_xor((int)(uint32_t)(u >> 32), off);
+      sum += __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+    }
+    top = max(top, (unsigned)__shfl_xor((int)top, off));
+  }
+  if (TPR == 64) return;
+  if ((threadIdx.x & 63) == 0) {
+    if (SUM) lds.sum[threadIdx.x >> 6] = sum;
+    lds.top[turn][threadIdx.x >> 6] = top;
+  }
   __syncthreads();
-  float s = 0.f;
+  top = 0;
 #pragma unroll
-  for (int i = 0; i < TPR / 64; ++i) s += red[i];
-  return s;
-}
-template <int TPR>
-__device__ __forceinline__ unsigned nq_max(unsigned v, unsigned* red) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, off));
-  if (TPR == 64) return v;
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  unsigned s = 0;
-#pragma unroll
-  for (int i = 0; i < TPR / 64; ++i) s = max(s, red[i]);
-  return s;
+  for (int i = 0; i < TPR / 64; ++i) top = max(top, lds.top[turn][i]);
+  if (SUM) {
+    sum = 0.;
+#pragma unroll 4  // (sixteen at once would be 32 registers)
+    for (int i = 0; i < TPR / 64; ++i) sum += lds.sum[i];
+  }
 }
 
 // TPR lanes per row, V steps of eight elements per lane: rows of up to 8 * TPR * V elements.
 template <int DT, int TPR, int V, bool NORM, bool RES, bool NT>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void hx_norm_int8_kernel(
     const typename NqT<DT>::T* __restrict__ x, long x_stride, const typename NqT<DT>::T* __restrict__ res, long res_stride,
-    const typename NqT<DT>::T* __restrict__ weight, float eps, typename NqT<DT>::T* __restrict__ h_out, signed char* __restrict__ q,
+    const typename NqT<DT>::T* __restrict__ weight, float eps, double by_width, typename NqT<DT>::T* __restrict__ h_out, signed char* __restrict__ q,
     float* __restrict__ scale, long rows, int width) {
   typedef typename NqT<DT>::T T;
   constexpr int RPW = TPR < 256 ? 256 / TPR : 1;  // rows per workgroup
-  __shared__ float red_sum[TPR / 64];
-  __shared__ unsigned red_max[TPR / 64];
+  __shared__ NqLds<TPR> lds;
   const long row = (long)blockIdx.x * RPW + (RPW > 1 ? threadIdx.x / TPR : 0);
   const int t = RPW > 1 ? threadIdx.x % TPR : threadIdx.x;
   if (row >= rows) return;  // (a whole wave leaves: with RPW > 1 a wave is a row and nothing below is shared)
@@ -118,43 +130,98 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void hx_norm_int8_kernel(
       nq_store(h_out + row * (long)width + at, width - at, h);
     }
   }
-  if (NORM) {
-    float ss = 0.f;
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-#pragma unroll
-      for (int e = 0; e < NQ_EPV; ++e) ss = fmaf(y[v][e], y[v][e], ss);
-    const float rms = sqrtf(nq_sum<TPR>(ss, red_sum) / (float)width + eps);
-    const float rstd = 1.f / rms;
+  double ss = 0.;
+  auto times_weight = [&](float unit, int t) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       float g[NQ_EPV];
       const int at = (v * TPR + t) * NQ_EPV;
       nq_load<false>(weight + at, width - at, g);
 #pragma unroll
-      for (int e = 0; e < NQ_EPV; ++e) y[v][e] = y[v][e] * rstd * g[e];
+      for (int e = 0; e < NQ_EPV; ++e) y[v][e] = y[v][e] * unit * g[e];
+      if (V >= 4) __builtin_amdgcn_sched_barrier(0);  // (the weights of all steps at once would not fit)
     }
+  };
+  auto largest = [&]() {  // the pattern of |y| as an integer: its order is that of the numbers, with infinity and NaN above them
+    unsigned top = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int e = 0; e < NQ_EPV; ++e) top = max(top, __float_as_uint(y[v][e]) & 0x7FFFFFFFu);
+    return top;
+  };
+  if (NORM) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int e = 0; e < NQ_EPV; ++e) ss = fma((double)y[v][e], (double)y[v][e], ss);
+    times_weight(1.f, t);
   }
-  // the pattern of |y| as an integer: its order is that of the numbers, with infinity and NaN above them
-  unsigned top = 0;
+  unsigned top = largest();
+  nq_join<TPR, NORM>(ss, top, lds, 0);
+  float unit = 1.f;  // the formula's y is what is in the registers / (unit * rms)
+  if (NORM && DT != HX_F16 && (top >= 0x7F800000u || (top < 0x0D800000u && ss > 0.))) {
+    // The largest product has left fp32 or come near its lower end (2^-100): once more, with a power of two near 1 / rms.
+    const uint64_t mean = __builtin_bit_cast(uint64_t, fma(ss, by_width, (double)eps));
+    const int e2 = 1023 - (int)((mean >> 52) & 0x7FF);
+    unit = __uint_as_float((uint32_t)(min(max(e2 >> 1, -126), 127) + 127) << 23);
+    int lane = t;
+    HX_OPAQUE_V(lane);  // (addresses of its own: those of the first loads would take their registers all along)
 #pragma unroll
-  for (int v = 0; v < V; ++v)
-#pragma unroll
-    for (int e = 0; e < NQ_EPV; ++e) top = max(top, __float_as_uint(y[v][e]) & 0x7FFFFFFFu);
-  top = nq_max<TPR>(top, red_max);
+    for (int v = 0; v < V; ++v) {
+      const int at = (v * TPR + lane) * NQ_EPV;
+      nq_load<false>((RES ? (const T*)h_out + row * (long)width : x + row * x_stride) + at, width - at, y[v]);
+      if (V >= 4) __builtin_amdgcn_sched_barrier(0);
+    }
+    times_weight(unit, lane);
+    top = largest();
+    nq_join<TPR, false>(ss, top, lds, 1);
+  }
   const float amax = __uint_as_float(top);
   const bool fine = top < 0x7F800000u && top != 0;
-  // a maximum so small that 127 / amax overflows is lifted by a power of two, and its row with it
-  const float lift = amax < 0x1p-100f ? 0x1p100f : 1.f;
-  const float inv = fine ? 127.f / (amax * lift) : 0.f;
-  if (t == 0) scale[row] = top == 0 ? 1.f : (top < 0x7F800000u ? amax / 127.f : amax);
+  // a maximum near either end of fp32 is moved from there by a power of two, and its row with it
+  const float lift = amax < 0x1p-100f ? 0x1p100f : amax > 0x1p100f ? 0x1p-100f : 1.f, most = fine ? amax * lift : 1.f, inv = 1.f / most;
+  // The quotient to the nearest integer.  127 times a product of two bf16 numbers, or an fp16 number, has at most 24 bits, and
+  // with the remainder of the first guess the fp32 quotient is the correctly rounded one: exact where it is a middle, and no
+  // other comes within 2^-24 of itself to one.  127 times a product of fp16 numbers or an fp32 number is rounded, the quotient
+  // off by less than 127 * 3 * 2^-24 < 2^-15, and where it lies that near to a middle (one in 2^14) it is worked out in fp64.
+  // (A product of fp32 numbers is rounded already.)
+  constexpr bool SHORT = DT == HX_BF16 || (DT == HX_F16) != NORM;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int at = (v * TPR + t) * NQ_EPV;
     signed char c[NQ_EPV];
+    float off = 0.f;
 #pragma unroll
-    for (int e = 0; e < NQ_EPV; ++e) c[e] = fine ? (signed char)(int)rintf(y[v][e] * lift * inv) : (signed char)0;
+    for (int e = 0; e < NQ_EPV; ++e) {
+      const float p = fine ? y[v][e] * lift * 127.f : 0.f;
+      float r = p * inv;
+      if (SHORT) r = fmaf(fmaf(-r, most, p), inv, r);
+      const float n = rintf(r);
+      c[e] = (signed char)(int)n;
+      if (!SHORT) off = fmaxf(off, fabsf(r - n));
+    }
+    if (V >= 4) __builtin_amdgcn_sched_barrier(0);
+    if (!SHORT && __builtin_amdgcn_ballot_w64(off > 0.5f - 0x1p-15f) != 0) {
+      const double by = 1. / (double)most;
+#pragma unroll
+      for (int e = 0; e < NQ_EPV; ++e) {
+        const double p = fine ? (double)(y[v][e] * lift) * 127. : 0.;
+        double r = p * by;
+        r = fma(fma(-r, (double)most, p), by, r);
+        c[e] = (signed char)(int)rint(r);
+        if (V >= 4) __builtin_amdgcn_sched_barrier(0);  // (one at a time: 8192 x 8192 fp16 56 -> 52 us)
+      }
+    }
     nq_store(q + row * (long)width + at, width - at, c);
+  }
+  if (t == 0) {  // (last: a chain of roots and quotients that nothing waits for)
+    if (NORM) {
+      const double rms = sqrt(fma(ss, by_width, (double)eps));
+      scale[row] = top == 0 && rms > 0. ? 1.f : (float)((double)amax / ((double)unit * rms * 127.));
+    } else {
+      scale[row] = top == 0 ? 1.f : (top < 0x7F800000u ? amax / 127.f : amax);
+    }
   }
 }
 
@@ -171,7 +238,7 @@ static void nq_launch(const void* x, long xs, const void* res, long rs, const vo
     for (long at = 0; at < rows; at += most) {
       const long n = rows - at < most ? rows - at : most;
       hx_launch(kernel, dim3((unsigned)((n + rpw - 1) / rpw)), dim3(tpr < 256 ? 256 : tpr), 0, s, (const T*)x + at * xs, xs,
-                RES ? (const T*)res + at * rs : nullptr, rs, (const T*)w, eps, RES ? (T*)h + at * width : nullptr,
+                RES ? (const T*)res + at * rs : nullptr, rs, (const T*)w, eps, 1. / width, RES ? (T*)h + at * width : nullptr,
                 (signed char*)q + at * width, scale + at, n, width);
     }
   };

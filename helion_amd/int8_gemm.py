@@ -32,7 +32,8 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
     """Root-mean-square norm over the last dimension with 8-bit output: ``(q, scale)`` of
     ``h * rsqrt(mean(h^2) + eps) * weight`` as in :func:`int8_quantize_per_token`, with ``h = x``; or, with a residual of x's
     shape, ``(q, scale, h)`` with ``h = x + residual`` rounded to x's dtype: the new residual, of whose rounded values the
-    norm is taken.  weight: [width] of x's dtype.  Everything behind h is fp32."""
+    norm is taken.  weight: [width] of x's dtype.  The mean of the squares is fp64; the integers are those of the formula for 16-bit
+    types (for float32 ``h * weight`` is rounded once), the scale is rounded once."""
     if residual is None:
         return rms_norm_int8_call(x, weight, eps)
     return add_rms_norm_int8_call(x, residual, weight, eps)

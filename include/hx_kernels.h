@@ -278,9 +278,10 @@ int hx_attention_path(int64_t BH, int64_t M, int64_t N, int64_t D, int dtype, co
 
 /* Row-wise quantisation to 8-bit integers, behind a root-mean-square norm or by itself:
  *   hx_rms_norm_int8:            h = round_T(x + residual) (h = x without a residual);
- *                                y = h * rsqrt(mean(h^2) + eps) * weight, in fp32
+ *                                y = h * rsqrt(mean(h^2) + eps) * weight
  *   hx_int8_quantize_per_token:  y = x
  *   both: scale[row] = max|y| / 127 (1 for a row of zeros), q = y * 127 / max|y| to the nearest integer, ties to even.
+ * The mean is fp64, the integers are exact for 16-bit types (h * weight is rounded once to fp32 for fp32), the scale is rounded once.
  * A row whose y holds a NaN or an infinity gets that as its scale and zeros as its integers (0 * scale is NaN).
  * x, residual: rows x width of `dtype` (HX_F16 / HX_BF16 / HX_F32), elements of a row contiguous, row strides in elements;
  * weight [width] of the same dtype; h_out (with a residual), q and scale are contiguous.  1 <= width <= 65536, any rows,

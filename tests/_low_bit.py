@@ -130,3 +130,34 @@ def cancelling_case(dtype, dim, page, kv_heads, group, lens, news):
     q = torch.zeros_like(q)
     q[..., 0] = (math.log(1.5) * dim**0.5 + 0.02 * torch.arange(q.shape[0] * q.shape[1]).view(q.shape[:2]).remainder(7)).to(dtype)
     return q, cache, table, n, start
+
+
+def border_rows(dtype, width, norm, seed=0):
+    """(x, weight): three rows whose values x * weight * 127 / max lie next to the middle between two integers, as near as
+    x's type allows, on it (a half of the maximum) and anywhere; weight is None without a norm"""
+    g = torch.Generator().manual_seed(seed)
+    w = (1 + 0.3 * torch.randn(width, generator=g)).to(dtype) if norm else torch.ones(width, dtype=dtype)
+    x = torch.randn(3, width, generator=g).to(dtype)
+    k = torch.randint(-126, 126, (2, width), generator=g) + 0.5
+    for row in range(2):
+        x[row, 0] = 5.3 + row
+        top = x[row, 0].double() * w[0].double()
+        for c in range(1, width):
+            best = (k[row, c] * top / 127 / w[c].double()).to(dtype)
+            if dtype != F32:  # of the numbers nearby the one whose quotient comes nearest to a middle
+                near = (best.view(torch.int16) + torch.arange(-200, 201, dtype=torch.int16)).view(dtype)
+                near = near[(near.double() * w[c].double()).abs() < top.abs()]
+                off = (near.double() * w[c].double() * 127 / top) % 1 - 0.5
+                best = near[off.abs().argmin()]
+            x[row, c] = best
+    if norm:
+        w[width // 2] = w[0]
+    x[:2, width // 2] = x[:2, 0] / 2
+    return x, w if norm else None
+
+
+def check_border_rows(q, x, weight):
+    """The integers of the formula: products of 16-bit numbers, and 127 times them, are exact in float64, so the quotient is
+    rounded once, by 2^-53 of itself, where the nearest one that is no middle is 2^-32 away."""
+    y = x.double() if weight is None else x.double() * weight.double()
+    assert torch.equal(q.double(), torch.round(y * 127 / y.abs().amax(-1, keepdim=True)))

@@ -546,3 +546,34 @@ def test_kv4_attention_weights_lose_nothing_to_a_batch(case, dim, page, kv_heads
 def _dev_case(case):
     q, cache, table, n, start = case
     return (q.to(DEV), hx.Kv4Cache(*_dev(*cache)), *_dev(table, n, start))
+
+
+# ---------------------------------------------------------------------------------------------- integers next to a border
+@pytest.mark.parametrize("dtype,width,norm", [(HF, 700, True), (BF, 300, True), (HF, 1500, True), (F32, 515, False), (HF, 64, False), (F32, 2100, False)])
+def test_integers_are_those_of_the_formula(dtype, width, norm):
+    x, w = lb.border_rows(dtype, width, norm)
+    q, _ = hx.rms_norm_int8(x.to(DEV), w.to(DEV)) if norm else hx.int8_quantize_per_token(x.to(DEV))
+    lb.check_border_rows(q.cpu(), x, w)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_a_prompt_has_the_integers_and_scales_of_the_formula(dtype):
+    """every integer of 2048 rows: products are exact, so only a quotient on a middle could differ, and both sides round it
+    to the even one; the scale is rounded once from 64 bits (an ulp for what the roots and sums of float64 differ by)"""
+    g = torch.Generator(DEV).manual_seed(0)
+    x, r = (torch.randn(2048, 8192, device=DEV, generator=g).to(dtype) for _ in range(2))
+    w = (1 + 0.2 * torch.randn(8192, device=DEV, generator=g)).to(dtype)
+    q, scale, h = hx.rms_norm_int8(x, w, residual=r)
+    want = ref.add(x, r)
+    assert torch.equal(h, want)
+    lb.check_border_rows(q, h, w)
+    exact = ref.row_scale(ref.rms_norm(h, w, 1e-6))
+    assert ((scale.double() - exact).abs() <= 2.0**-24 * (1 + 1e-6) * exact).all()
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-20, 1e25, 3e38])
+def test_rms_norm_int8_squares_beyond_fp32(size):
+    x, _, w = lb.norm_inputs(3, 5000, F32, False, 7)
+    x = x / x.abs().amax(-1, keepdim=True).clamp(min=1) * size
+    q, scale = hx.rms_norm_int8(x.to(DEV), w.to(DEV))
+    lb.check_rows(q.cpu(), scale.cpu(), ref.rms_norm(x, w, 1e-6), 4)

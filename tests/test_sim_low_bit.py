@@ -257,3 +257,20 @@ def test_kv4_attention_weights_lose_nothing_to_a_batch(case, dtype, dim, page, k
     with simlib.cus(cus):
         out = simops.kv4_attention(q, cache, table, n, start)
     lb.check_attention(out, q, cache, table, n, start, p_terms=2)
+
+
+# ---------------------------------------------------------------------------------------------- integers next to a border
+@pytest.mark.parametrize("dtype,width,norm", [(HF, 700, True), (BF, 300, True), (F32, 515, False), (HF, 64, False)])
+def test_integers_are_those_of_the_formula(dtype, width, norm):
+    x, w = lb.border_rows(dtype, width, norm)
+    q, _, _ = simops.rms_norm_int8(x, w)
+    lb.check_border_rows(q, x, w)
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-20, 1e25, 3e38])
+def test_rms_norm_int8_squares_beyond_fp32(size):
+    """the mean of the squares is in 64 bits: rows whose squares leave fp32 are like others (eps: 1e-6)"""
+    x, _, w = lb.norm_inputs(3, 130, F32, False, 7)
+    x = x / x.abs().amax(-1, keepdim=True).clamp(min=1) * size
+    q, scale, _ = simops.rms_norm_int8(x, w)
+    lb.check_rows(q, scale, ref.rms_norm(x, w, 1e-6), 4)
