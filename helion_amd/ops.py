@@ -741,16 +741,20 @@ matmul_call = _caller(_matmul_impl, matmul_op)
 attention_call = _caller(_attention_impl, attention_op)
 
 
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
 def _light_caller(impl, op, tensors):
-    """As _caller, for calls whose first `tensors` arguments are the tensors (or None): these are all it looks at."""
+    """As _caller, for calls whose first `tensors` arguments are the tensors (or None): these are all it looks at.  A module's
+    weights count as plain, and since no result carries a gradient, arguments that require one are passed on without."""
     def call(*args):
         if not torch.compiler.is_compiling():
             for t in args[:tensors]:
-                if t is not None and (type(t) is not torch.Tensor or not t.is_cuda):
+                if t is not None and (type(t) not in _PLAIN or not t.is_cuda):
                     break
             else:
                 return impl(*args)
-        return op(*args)
+        return op(*(t.detach() if isinstance(t, torch.Tensor) and t.requires_grad else t for t in args))
     return call
 
 

@@ -577,3 +577,16 @@ def test_rms_norm_int8_squares_beyond_fp32(size):
     x = x / x.abs().amax(-1, keepdim=True).clamp(min=1) * size
     q, scale = hx.rms_norm_int8(x.to(DEV), w.to(DEV))
     lb.check_rows(q.cpu(), scale.cpu(), ref.rms_norm(x, w, 1e-6), 4)
+
+
+# ---------------------------------------------------------------------------------------------- weights of a module
+def test_a_modules_weight_is_a_plain_argument():
+    """an nn.Parameter (the usual norm weight or bias) gives what its data gives and leaves no graph"""
+    x, w = torch.randn(6, 128, device=DEV).to(BF), torch.randn(128, device=DEV).to(BF)
+    a, b, sa, sb, bias = _dev(*lb.gemm_inputs(6, 16, 128, 0, BF))
+    call = lambda x, w, bias: (*hx.rms_norm_int8(x, w), *hx.rms_norm_int8(x, w, residual=x), *hx.int8_quantize_per_token(x),
+                               hx.int8_gemm(a, b, sa, sb, bias=bias))
+    want = call(x, w, bias)
+    for run in (call, torch.compile(call, backend="eager", fullgraph=True)):
+        got = run(x.clone().requires_grad_(), torch.nn.Parameter(w), torch.nn.Parameter(bias))
+        assert all(torch.equal(i, j) and not i.requires_grad for i, j in zip(got, want))

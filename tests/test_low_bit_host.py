@@ -156,3 +156,19 @@ def test_restatement_of_the_format():
     assert vc.shape == (3, 2, 4, 16, 4, 2) and vs.shape == (3, 2, 4, 2, 4)
     # piece 5 of token 6 of a head: elements 20 .. 23
     assert vc[1, 0, 1, 5, 2].tolist() == [int(c[1, 0, 6, 20] | c[1, 0, 6, 21] << 4), int(c[1, 0, 6, 22] | c[1, 0, 6, 23] << 4)]
+
+
+def test_a_modules_weight_and_inputs_that_require_grad_leave_no_graph():
+    """no result carries a gradient, whichever of the arguments would"""
+    m = lambda *s, dt=torch.bfloat16: torch.empty(s, dtype=dt, device="meta")
+    weight = torch.nn.Parameter(m(64))
+    x = m(5, 64).requires_grad_()
+    f32 = lambda n: m(n, dt=torch.float32).requires_grad_()
+    a8, b8 = m(5, 64, dt=torch.int8), m(64, 8, dt=torch.int8)
+    c = hx.kv4_cache(3, 16, 2, 64, device="meta")
+    kv, q, i32 = m(4, 2, 64).requires_grad_(), m(4, 6, 64).requires_grad_(), lambda *s: m(*s, dt=torch.int32)
+    results = [*hx.rms_norm_int8(m(5, 64), weight), *hx.rms_norm_int8(x, weight, residual=m(5, 64)), *hx.rms_norm_int8(x, m(64), residual=x),
+               *hx.int8_quantize_per_token(x), hx.int8_gemm(a8, b8, f32(5), f32(8), bias=torch.nn.Parameter(m(8))),
+               *hx.kv4_read(c, m(5, dt=torch.int64)), hx.kv4_attention(q, c, i32(4, 2), i32(4)), hx.kv4_attention(q, c, i32(4, 2), i32(4), out=m(4, 6, 64))]
+    hx.kv4_write(c, kv, kv, m(4, dt=torch.int64))
+    assert not any(t.requires_grad for t in (*results, *c))
