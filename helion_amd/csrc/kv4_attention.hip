@@ -573,9 +573,10 @@ struct KaPlan {
   bool many;  // hx_kv4_attention_rows
 };
 
-static KaPlan ka_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t max_query, int64_t max_keys, int dt) {
+static KaPlan ka_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t max_query, int64_t max_keys, int dt) {
   KaPlan p;
-  const int64_t rows = max_query * (heads / kv_heads);
+  // (a max_query that is padded, for a graph or by a server's limit, plans what the tokens need)
+  const int64_t rows = (max_query < tokens ? max_query : tokens) * (heads / kv_heads);
   // Two blocks of rows share a conversion of the keys and values; a head dim of 256 or an fp32 query leaves no registers for it.
   p.rb = rows > 16 && D <= 128 && dt != HX_F32 ? 2 : 1;
   p.nw = 4;
@@ -632,7 +633,7 @@ static int ka_check_sizes(const char* who, int64_t tokens, int64_t batch, int64_
 extern "C" size_t hx_kv4_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t page,
                                                    int64_t table_width, int64_t max_query, int dtype) {
   if (tokens <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || D <= 0) return 0;
-  const KaPlan p = ka_plan(batch, heads, kv_heads, D, max_query, table_width * page, dtype);
+  const KaPlan p = ka_plan(tokens, batch, heads, kv_heads, D, max_query, table_width * page, dtype);
   return p.splits == 1 ? 0 : (size_t)tokens * heads * p.splits * (D + 2) * sizeof(float);
 }
 
@@ -677,7 +678,7 @@ extern "C" int hx_kv4_attention(const void* q, int64_t q_token_stride, int64_t q
     hx_set_error("%s: out must be 16-byte aligned, the other pointers aligned to their elements", who);
     return HX_ERR_UNSUPPORTED;
   }
-  const KaPlan p = ka_plan(batch, heads, kv_heads, D, query_start ? max_query : 1, table_width * page, dtype);
+  const KaPlan p = ka_plan(tokens, batch, heads, kv_heads, D, query_start ? max_query : 1, table_width * page, dtype);
   const size_t need = p.splits == 1 ? 0 : (size_t)tokens * heads * p.splits * (D + 2) * sizeof(float);
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) {
     hx_set_error("%s: workspace must be 16-byte aligned and at least %zu bytes (got %zu)", who, need, workspace_bytes);

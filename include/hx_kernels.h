@@ -333,8 +333,8 @@ int hx_kv4_read(const void* k_codes, const void* k_scales, const void* v_codes, 
  * A row that sees no key gives zeros.  Rows of q outside every sequence are neither read nor written.  Table entries behind
  * the last page of a sequence are not used; the keys of a page that does not exist are masked, as are lengths beyond the table.
  * q [tokens][heads][D] of `dtype`, elements of a head contiguous, token and head strides in elements; out contiguous,
- * 16-byte aligned, same dtype.  max_query: the most new tokens of one sequence (sizes the launch; more are computed too,
- * only slower).  Products of exact bf16 terms (1 for a bf16 q, 2 for fp16, 3 for fp32), fp32 sums and statistics.
+ * 16-byte aligned, same dtype.  max_query: the most new tokens of one sequence (sizes the launch, with `tokens` as its
+ * limit, 1 where query_start is NULL; more are computed too, only slower).  Products of exact bf16 terms (1 for a bf16 q, 2 for fp16, 3 for fp32), fp32 sums and statistics.
  * workspace: hx_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned (0 where the keys are not split). */
 int hx_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_codes, const void* k_scales,
                      const void* v_codes, const void* v_scales, const int32_t* block_table, int64_t table_stride,

@@ -172,3 +172,16 @@ def test_a_modules_weight_and_inputs_that_require_grad_leave_no_graph():
                *hx.kv4_read(c, m(5, dt=torch.int64)), hx.kv4_attention(q, c, i32(4, 2), i32(4)), hx.kv4_attention(q, c, i32(4, 2), i32(4), out=m(4, 6, 64))]
     hx.kv4_write(c, kv, kv, m(4, dt=torch.int64))
     assert not any(t.requires_grad for t in (*results, *c))
+
+
+def test_a_padded_max_query_plans_what_the_tokens_need():
+    """max_query sizes the launch, but no sequence has more new tokens than there are: one token over 32768 keys is split as
+    ever, and no count is too large"""
+    lib = _lib.load()
+    need = lambda tokens, mq: lib.hx_kv4_attention_workspace_bytes(tokens, 1, 64, 8, 128, 64, 512, mq, 1)
+    assert need(1, 1) > 0
+    assert need(1, 4096) == need(1, 2**62) == need(1, 1)
+    assert need(4, 4096) == need(4, 4) > 0
+    ab = dict(q=A, qt=8192, qh=128, kc=A, ks=A, vc=A, vs=A, table=A, ts=512, lens=A, start=A, out=A, tokens=1, batch=1, heads=64, kv=8, D=128,
+              pages=512, page=64, width=512, mq=4096, scale=0.1, causal=1, dt=1, ws=A, wsb=need(1, 1) - 1)
+    assert lib.hx_kv4_attention(*ab.values(), None) == -3 and str(need(1, 1)).encode() in lib.hx_last_error()  # the same plan
