@@ -21,11 +21,19 @@ def _stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_dispatch_modes = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 0)
+
+
+def _watched() -> bool:
+    """Does something want to see the ops: torch.compile, or a dispatch mode (make_fx, a flop counter, a log)?"""
+    return torch.compiler.is_compiling() or _dispatch_modes() > 0
+
+
 def eager(op_impl, op, *args):
     """Call the op's implementation directly for plain CUDA tensors in eager mode (the dispatcher round trip of a
     custom op costs more than a small kernel), and through the registered op when tracing / compiling or for anything
     else (fake or meta tensors get shape inference there, CPU tensors their error)."""
-    if not torch.compiler.is_compiling() and all(type(a) is torch.Tensor and a.is_cuda for a in args if isinstance(a, torch.Tensor)):
+    if not _watched() and all(type(a) is torch.Tensor and a.is_cuda for a in args if isinstance(a, torch.Tensor)):
         return op_impl(*args)
     return op(*args)
 
@@ -748,7 +756,7 @@ def _light_caller(impl, op, tensors):
     """As _caller, for calls whose first `tensors` arguments are the tensors (or None): these are all it looks at.  A module's
     weights count as plain, and since no result carries a gradient, arguments that require one are passed on without."""
     def call(*args):
-        if not torch.compiler.is_compiling():
+        if not _watched():
             for t in args[:tensors]:
                 if t is not None and (type(t) not in _PLAIN or not t.is_cuda):
                     break

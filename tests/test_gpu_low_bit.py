@@ -590,3 +590,35 @@ def test_a_modules_weight_is_a_plain_argument():
     for run in (call, torch.compile(call, backend="eager", fullgraph=True)):
         got = run(x.clone().requires_grad_(), torch.nn.Parameter(w), torch.nn.Parameter(bias))
         assert all(torch.equal(i, j) and not i.requires_grad for i, j in zip(got, want))
+
+
+# ---------------------------------------------------------------------------------------------- dispatch modes
+def test_dispatch_modes_see_the_operators():
+    """a mode (here a log, and make_fx's) sees the registered ops, and what it traces computes the same"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    seen = []
+
+    class Log(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(func.name())
+            return func(*args, **(kwargs or {}))
+
+    x, w = torch.randn(6, 128, device=DEV).to(BF), torch.randn(128, device=DEV).to(BF)
+    b, sb = hx.int8_quantize_per_token(torch.randn(32, 128, device=DEV).to(BF))
+
+    def step(x):
+        q, s, h = hx.rms_norm_int8(x, w, residual=x)
+        return hx.int8_gemm(q, b.t(), s, sb), h, hx.matmul(x, w.view(128, 1).expand(128, 8).contiguous())
+
+    want = step(x)
+    with Log():
+        got = step(x)
+    assert all(torch.equal(i, j) for i, j in zip(got, want))
+    names = {"helion_amd::add_rms_norm_int8", "helion_amd::int8_gemm", "helion_amd::matmul"}
+    assert names <= set(seen)
+    traced = make_fx(step)(x)
+    assert names <= {str(n.target).replace(".default", "").replace(".", "::") for n in traced.graph.nodes}
+    y = torch.randn_like(x)
+    assert all(torch.equal(i, j) for i, j in zip(traced(y), step(y)))
