@@ -169,7 +169,9 @@ __device__ __forceinline__ void ka_queries(const KaArgs& a, const KaSeq& q, int 
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         __bf16 t[NQ];
-        ka_terms<NQ>(a.negate ? -(float)raw[e] : (float)raw[e], t);
+        // (an infinity becomes NaN: it makes its row that, but every score of it may be minus infinity, as for a row without a key)
+        const float f = __builtin_fmaf((float)raw[e], 0.f, (float)raw[e]);
+        ka_terms<NQ>(a.negate ? -f : f, t);
 #pragma unroll
         for (int n = 0; n < NQ; ++n) qf[rb][n][m][e] = t[n];
       }

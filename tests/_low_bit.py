@@ -161,3 +161,15 @@ def check_border_rows(q, x, weight):
     rounded once, by 2^-53 of itself, where the nearest one that is no middle is 2^-32 away."""
     y = x.double() if weight is None else x.double() * weight.double()
     assert torch.equal(q.double(), torch.round(y * 127 / y.abs().amax(-1, keepdim=True)))
+
+
+def infinite_queries(dtype, group, news, kv_heads=1):
+    """Sequences of 3 and 33 keys in turn (the first ones' first tokens see none) whose keys all have a positive first element;
+    -inf there in token 0, which sees nothing, and token 3, inf in token 6."""
+    lens = [3, 33] * (len(news) // 2)
+    q, cache, table, n, start = attention_case(dtype, 64, 16, kv_heads, group, lens, news)
+    codes, scales = ref.from_layout(cache[0], cache[1], False)
+    codes[..., 0] = 4
+    cache = (*ref.to_layout(codes, scales, False), *cache[2:])
+    q[[0, 3], :, 0], q[6, :, 0] = -math.inf, math.inf
+    return q, cache, table, lens, start, n

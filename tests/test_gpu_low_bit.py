@@ -622,3 +622,14 @@ def test_dispatch_modes_see_the_operators():
     assert names <= {str(n.target).replace(".default", "").replace(".", "::") for n in traced.graph.nodes}
     y = torch.randn_like(x)
     assert all(torch.equal(i, j) for i, j in zip(traced(y), step(y)))
+
+
+# ---------------------------------------------------------------------------------------------- infinities in q
+@pytest.mark.parametrize("dtype,group,kv_heads,pairs", [(BF, 2, 1, 1), (HF, 8, 2, 1), (BF, 16, 64, 4), (F32, 2, 1, 1)])
+def test_kv4_attention_of_infinite_queries(dtype, group, kv_heads, pairs):
+    """an infinity in q makes the row NaN, also where it takes every score to minus infinity; a row without a key stays zero"""
+    q, cache, table, _, start, n = lb.infinite_queries(dtype, group, [5, 7] * pairs, kv_heads)
+    cd = hx.Kv4Cache(*_dev(*cache))
+    out = hx.kv4_attention(q.to(DEV), cd, table.to(DEV), n.to(DEV), query_start=start.to(DEV), max_query_len=7).cpu()
+    lb.check_attention(out, q, cache, table, n, start)
+    assert torch.isnan(out[3]).all() and (out[0] == 0).all() and torch.isnan(out[6]).all()

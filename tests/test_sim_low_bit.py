@@ -274,3 +274,13 @@ def test_rms_norm_int8_squares_beyond_fp32(size):
     x = x / x.abs().amax(-1, keepdim=True).clamp(min=1) * size
     q, scale, _ = simops.rms_norm_int8(x, w)
     lb.check_rows(q, scale, ref.rms_norm(x, w, 1e-6), 4)
+
+
+@pytest.mark.parametrize("dtype,group,news,cus", [(BF, 2, [5, 7], 256), (HF, 8, [5, 7], 256), (BF, 16, [5, 7], 1), (F32, 2, [5, 7], 256)])
+def test_kv4_attention_of_infinite_queries(dtype, group, news, cus):
+    """an infinity in q makes the row NaN, also where it takes every score to minus infinity; a row without a key stays zero"""
+    q, cache, table, _, start, n = lb.infinite_queries(dtype, group, news)
+    with simlib.cus(cus):
+        out = simops.kv4_attention(q, cache, table, n, start)
+    lb.check_attention(out, q, cache, table, n, start)
+    assert torch.isnan(out[3, :, :]).all() and (out[0] == 0).all() and torch.isnan(out[6]).all()
