@@ -102,6 +102,7 @@ _SIGNATURES = {
         [_c.c_void_p] * 3 + [_c.c_int64] * 7 + [_c.c_void_p] * 3 + [_c.c_int, _c.c_int, _c.c_void_p, _c.c_size_t, _c.c_void_p],
     ),
     "hx_int8_gemm_workspace_bytes": (_c.c_size_t, [_c.c_int64] * 6 + [_c.c_void_p] * 2),
+    "hx_int8_gemm_path": (_c.c_int, [_c.c_int64] * 6 + [_c.c_void_p] * 2),
     "hx_kv4_write": (_c.c_int, [_c.c_void_p] * 7 + [_c.c_int] + [_c.c_int64] * 9 + [_c.c_int, _c.c_void_p]),
     "hx_kv4_read": (_c.c_int, [_c.c_void_p] * 5 + [_c.c_int] + [_c.c_void_p] * 2 + [_c.c_int64] * 5 + [_c.c_int, _c.c_void_p]),
     "hx_kv4_attention": (
@@ -110,6 +111,7 @@ _SIGNATURES = {
         + [_c.c_float, _c.c_int, _c.c_int, _c.c_void_p, _c.c_size_t, _c.c_void_p],
     ),
     "hx_kv4_attention_workspace_bytes": (_c.c_size_t, [_c.c_int64] * 8 + [_c.c_int]),
+    "hx_kv4_attention_path": (_c.c_int, [_c.c_int64] * 8 + [_c.c_int]),
     "hx_clock_probe": (_c.c_int, [_c.c_void_p, _c.c_int64, _c.c_void_p]),
     "hx_matmul_path": (_c.c_int, [_c.c_int64] * 7 + [_c.c_int, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p]),
 }

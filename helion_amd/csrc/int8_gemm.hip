@@ -667,6 +667,12 @@ extern "C" size_t hx_int8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, 
   return i8_plan(M, N, K, lda, ldb_k, ldb_n, ((uintptr_t)a & 15) == 0, ((uintptr_t)b & 15) == 0).bytes;
 }
 
+extern "C" int hx_int8_gemm_path(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb_k, int64_t ldb_n, const void* a, const void* b) {
+  if (M <= 0 || N <= 0 || K <= 0 || i8_check("hx_int8_gemm", M, N, K) != 0) return 0;
+  const I8Plan p = i8_plan(M, N, K, lda, ldb_k, ldb_n, ((uintptr_t)a & 15) == 0, ((uintptr_t)b & 15) == 0);
+  return (p.ns >= 0 ? 1 : p.bm == 64 ? 2 : p.bm == 128 ? 3 : 4) + (p.splits > 1 ? 8 : 0) + (p.tail ? 16 : 0);
+}
+
 static void i8_pack(const void* src, uint8_t* dst, int64_t rows, int64_t K, int64_t sr, int64_t sk, int64_t ld, hipStream_t s) {
   if (sk == 1)
     hx_launch(hx_int8_pack_rows, dim3((unsigned)((rows * (ld / 16) + 255) / 256)), dim3(256), 0, s, (const uint8_t*)src, dst, (long)rows, (int)K,

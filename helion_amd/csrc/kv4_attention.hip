@@ -639,6 +639,13 @@ extern "C" size_t hx_kv4_attention_workspace_bytes(int64_t tokens, int64_t batch
   return p.splits == 1 ? 0 : (size_t)tokens * heads * p.splits * (D + 2) * sizeof(float);
 }
 
+extern "C" int hx_kv4_attention_path(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t page,
+                                     int64_t table_width, int64_t max_query, int dtype) {
+  if (tokens <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || D <= 0) return 0;
+  const KaPlan p = ka_plan(tokens, batch, heads, kv_heads, D, max_query, table_width * page, dtype);
+  return (p.many ? 3 : p.rb) + (p.splits > 1 ? 8 : 0);
+}
+
 template <int D, int DT>
 static void ka_launch(const KaArgs& a, const KaPlan& p, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.kv_heads * a.batch * p.splits * p.blocks)), block(p.nw * 64);  // (at most KA_GRID)

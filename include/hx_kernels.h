@@ -304,6 +304,9 @@ int hx_int8_gemm(const void* a, const void* b, void* c, int64_t M, int64_t N, in
                  void* workspace, size_t workspace_bytes, void* stream);
 size_t hx_int8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb_k, int64_t ldb_n, const void* a,
                                     const void* b);
+/* Which kernel a call runs: 1 = up to 32 rows, 2, 3, 4 = tiles of 64, 128, 256 rows; 8 more where K is split over workgroups, 16
+ * more where K % 128 != 0 and an operand is read in place; 0 = none (an empty or refused size). */
+int hx_int8_gemm_path(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb_k, int64_t ldb_n, const void* a, const void* b);
 
 /* A key/value cache held in 4 bits (the open MXFP4 format: e2m1 elements, a power-of-two scale for each 32 of a head).
  * D = 64, 128 or 256; pages of `page` tokens, a power of two from 16 to 1024; slot = page index * page + place in it.
@@ -343,6 +346,10 @@ int hx_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_strid
                      int causal, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 size_t hx_kv4_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t page,
                                         int64_t table_width, int64_t max_query, int dtype);
+/* Which kernel a call runs: 1, 2, 3 = 16, 32, 128 rows (a new token of one query head) a workgroup; 8 more where the keys are
+ * split over workgroups; 0 = none (an empty size). */
+int hx_kv4_attention_path(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t page, int64_t table_width,
+                          int64_t max_query, int dtype);
 
 /* ---- Diagnostics (not part of the drop-in interface; no counterpart in the reference) --------------------------------
  * One wave that measures the engine clock of the XCD it lands on as (shader-clock counter delta) / (100 MHz counter

@@ -633,3 +633,36 @@ def test_kv4_attention_of_infinite_queries(dtype, group, kv_heads, pairs):
     out = hx.kv4_attention(q.to(DEV), cd, table.to(DEV), n.to(DEV), query_start=start.to(DEV), max_query_len=7).cpu()
     lb.check_attention(out, q, cache, table, n, start)
     assert torch.isnan(out[3]).all() and (out[0] == 0).all() and torch.isnan(out[6]).all()
+
+
+# ---------------------------------------------------------------------------------------------- every kernel, by its path
+@pytest.mark.parametrize("m,n,k,bias,out,path", [
+    (512, 4096, 4096, BF, BF, 2), (200, 515, 48, HF, BF, 18), (100, 512, 16000, BF, BF, 10), (130, 2048, 16400, None, HF, 26),
+    (777, 4096, 4096, BF, BF, 3), (777, 4100, 4112, F32, HF, 19), (200, 4096, 16384, BF, BF, 11), (200, 4096, 16400, HF, HF, 27),
+    (3500, 2560, 4096, BF, BF, 4), (3500, 2500, 4096, HF, F32, 4), (3500, 2560, 4112, F32, HF, 20),
+    (1, 256, 128, None, HF, 1), (16, 1024, 8192, BF, BF, 9), (16, 300, 1040, F32, F32, 17), (30, 64, 9008, HF, BF, 25),
+])
+def test_int8_gemm_every_kernel(m, n, k, bias, out, path):
+    """tiles of 64, 128 and 256 rows and the kernel for up to 32, unsplit and split, K a multiple of 128 and not, the output types"""
+    from helion_amd import _lib
+
+    x, y, sa, sb, b = _dev(*lb.gemm_inputs(m, n, k, m + n + k, bias))
+    assert _lib.load().hx_int8_gemm_path(m, n, k, k, 1, k, x.data_ptr(), y.data_ptr()) == path
+    lb.check_gemm(hx.int8_gemm(x, y, sa, sb, bias=b, out_dtype=out), x, y, sa, sb, b, out)
+
+
+@pytest.mark.parametrize("dtype,dim,page,kv_heads,group,lens,news,path", [
+    (BF, 128, 64, 8, 8, [300 + 10 * i for i in range(32)], [64] * 32, 3), (BF, 64, 16, 8, 8, [300 + 10 * i for i in range(32)], [64 - i for i in range(32)], 3),
+    (HF, 128, 32, 8, 8, [600 - 10 * i for i in range(32)], [64] * 32, 3), (BF, 128, 32, 8, 4, [700, 65] * 4, [100, 1] * 4, 2),
+    (BF, 128, 64, 8, 8, [5000, 20], None, 9), (BF, 64, 16, 2, 8, [4100], [4], 10), (BF, 128, 16, 8, 4, [200], None, 1),
+])
+def test_kv4_attention_every_kernel(dtype, dim, page, kv_heads, group, lens, news, path):
+    """16, 32 and 128 rows a workgroup, keys split and not; maxima that move over the tiles"""
+    from helion_amd import _lib
+
+    q, cache, table, n, start = _dev_case(lb.attention_case(dtype, dim, page, kv_heads, group, lens, news))
+    q = q * torch.linspace(0.2, 3, q.shape[0], device=DEV)[:, None, None].to(dtype)
+    mq = max(news) if news else 1
+    assert _lib.load().hx_kv4_attention_path(q.shape[0], len(lens), q.shape[1], kv_heads, dim, page, table.shape[1], mq, 1 if dtype == BF else 0) == path
+    out = hx.kv4_attention(q, cache, table, n, query_start=start, max_query_len=mq)
+    lb.check_attention(out, q, cache, table, n, start)

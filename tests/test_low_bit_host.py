@@ -185,3 +185,17 @@ def test_a_padded_max_query_plans_what_the_tokens_need():
     ab = dict(q=A, qt=8192, qh=128, kc=A, ks=A, vc=A, vs=A, table=A, ts=512, lens=A, start=A, out=A, tokens=1, batch=1, heads=64, kv=8, D=128,
               pages=512, page=64, width=512, mq=4096, scale=0.1, causal=1, dt=1, ws=A, wsb=need(1, 1) - 1)
     assert lib.hx_kv4_attention(*ab.values(), None) == -3 and str(need(1, 1)).encode() in lib.hx_last_error()  # the same plan
+
+
+def test_which_kernel_a_size_runs():
+    """(at 256 compute units, which is what the library takes without a GPU)"""
+    lib = _lib.load()
+    gemm = lambda m, n, k, a=A, b=A: lib.hx_int8_gemm_path(m, n, k, k, 1, k, a, b)
+    assert [gemm(*s) for s in ((16, 28672, 8192), (1, 64, 16384), (16, 300, 1040), (512, 4096, 4096), (128, 8192, 8192), (777, 4096, 4096),
+                               (777, 4100, 4112), (200, 4096, 16384), (8192, 8192, 8192), (3500, 2560, 4112))] == [1, 9, 17, 2, 10, 3, 19, 11, 4, 20]
+    assert gemm(8192, 8192, 8191) == 4 and gemm(777, 4100, 4112, A + 1) == 19 and gemm(777, 4100, 4112, A + 1, A + 1) == 3  # copies have whole k-tiles
+    assert gemm(0, 4, 4) == 0 and gemm(4, 4, 200000) == 0
+    att = lambda t, b, h, kv, d, page, width, mq, dt=1: lib.hx_kv4_attention_path(t, b, h, kv, d, page, width, mq, dt)
+    assert att(1, 1, 32, 8, 128, 16, 33, 1) == 1 and att(32, 32, 64, 8, 128, 64, 512, 1) == 9 and att(64, 64, 32, 32, 64, 16, 128, 1) == 1
+    assert att(2048, 1, 32, 8, 128, 64, 160, 2048) == 3 and att(1000, 24, 32, 8, 128, 32, 125, 200) == 2
+    assert att(2048, 1, 32, 8, 128, 64, 160, 2048, 2) == 1 and att(0, 1, 8, 8, 64, 16, 1, 1) == 0

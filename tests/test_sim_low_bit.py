@@ -245,8 +245,8 @@ def test_kv4_attention_no_pages():
 
 
 # (dtype, dim, page, kv_heads, group, lens, new tokens, compute units): 32 rows a workgroup, and 128
-WEIGHTS = [(BF, 128, 16, 1, 8, [90, 33], [5, 4], 256), (BF, 64, 32, 1, 20, [70], None, 256), (BF, 128, 16, 1, 4, [90, 70], [33, 4], 1),
-           (BF, 64, 16, 1, 3, [129], [64], 1)]
+WEIGHTS = [(BF, 128, 16, 1, 8, [90, 33], [5, 4], 256), (BF, 64, 32, 1, 20, [70], None, 256), (BF, 128, 16, 1, 4, [90, 70], [32, 4], 1),
+           (BF, 64, 16, 2, 2, [129], [64], 1)]
 
 
 @pytest.mark.parametrize("dtype,dim,page,kv_heads,group,lens,news,cus", WEIGHTS)
@@ -284,3 +284,79 @@ def test_kv4_attention_of_infinite_queries(dtype, group, news, cus):
         out = simops.kv4_attention(q, cache, table, n, start)
     lb.check_attention(out, q, cache, table, n, start)
     assert torch.isnan(out[3, :, :]).all() and (out[0] == 0).all() and torch.isnan(out[6]).all()
+
+
+# ---------------------------------------------------------------------------------------------- every kernel of the product
+# (compute units, m, n, k, bias, out, path): tiles of 64, 128 and 256 rows, unsplit and split, K a multiple of 128 and not
+TILES = [
+    (1, 257, 257, 1040, BF, BF, 20), (1, 300, 513, 784, HF, F32, 20), (1, 129, 256, 640, None, HF, 4), (1, 129, 256, 2048, BF, BF, 4),
+    (4, 129, 256, 2064, F32, HF, 19), (4, 129, 256, 2048, BF, BF, 3), (3, 128, 128, 4096, BF, BF, 11), (8, 130, 128, 8208, None, HF, 27),
+    (16, 250, 250, 4112, F32, BF, 26), (4, 100, 128, 4096, None, F32, 10), (2, 128, 128, 4096, HF, HF, 2), (2, 100, 128, 2064, None, BF, 18),
+    (1, 5, 40, 8192, BF, BF, 1), (4, 5, 40, 8192, None, HF, 9), (1, 20, 40, 8208, F32, F32, 25), (256, 20, 70, 1040, HF, BF, 17),
+]
+
+
+@pytest.mark.parametrize("cus,m,n,k,bias,out,path", TILES)
+@pytest.mark.parametrize("variant", ["lazy-reverse", "eager"])
+def test_int8_gemm_every_kernel(cus, m, n, k, bias, out, path, variant):
+    simlib.configure(variant)
+    x, y, sa, sb, b = lb.gemm_inputs(m, n, k, m + n + k, bias)
+    A = 1 << 20
+    with simlib.cus(cus):
+        assert simlib.load().hx_int8_gemm_path(m, n, k, k, 1, k, A, A) == path
+        got = simops.int8_gemm(x, y, sa, sb, b, out)
+    lb.check_gemm(got, x, y, sa, sb, b, out)
+
+
+def _path(q, cache, table, news):
+    pages, kv_heads, page, half = cache[0].shape
+    return simlib.load().hx_kv4_attention_path(q.shape[0], table.shape[0], q.shape[1], kv_heads, 2 * half, page, table.shape[1],
+                                               max(news) if news else 1, {HF: 0, BF: 1, F32: 2}[q.dtype])
+
+
+@pytest.mark.parametrize("cus,case,path", [
+    (256, (BF, 128, 16, 1, 8, [90, 33], [5, 4]), 2), (256, (BF, 128, 64, 1, 8, [40], None), 1), (256, (BF, 256, 16, 1, 8, [90, 33], [5, 4]), 1),
+    (256, (F32, 64, 16, 1, 8, [90, 33], [5, 4]), 1), (4, (BF, 64, 256, 1, 2, [2100, 130], None), 9), (4, (HF, 64, 256, 1, 2, [2100], [20]), 10),
+    # 128 rows a workgroup: sequences of 128 rows, 80, none, 4 and 16; several tiles of 64 keys; two and one workgroups of a sequence
+    (1, (BF, 128, 16, 1, 4, [200, 20, 0, 1, 70, 40], [32, 20, 0, 1, 4, 4]), 3), (1, (BF, 128, 32, 2, 8, [333, 150], [16, 9]), 3),
+    (1, (HF, 64, 16, 1, 4, [260, 150], [32, 20]), 3), (1, (HF, 128, 64, 2, 1, [300], [256]), 3), (1, (BF, 64, 16, 2, 2, [64, 129], [64, 1]), 3),
+])
+@pytest.mark.parametrize("causal", [True, False])
+def test_kv4_attention_every_kernel(cus, case, path, causal):
+    """the kernel a case runs; maxima that move over the tiles, both buffers, pages ahead of their use"""
+    q, cache, table, n, start = lb.attention_case(*case)
+    q = q * torch.linspace(0.2, 3, q.shape[0])[:, None, None].to(q.dtype)
+    with simlib.cus(cus):
+        assert _path(q, cache, table, case[6]) == path
+        out = simops.kv4_attention(q, cache, table, n, start, causal=causal)
+    lb.check_attention(out, q, cache, table, n, start, causal=causal, p_terms=3 if q.dtype == F32 else 2)
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF, 64), (HF, 128)])
+def test_kv4_attention_masks_with_128_rows_a_workgroup(dtype, dim):
+    """rows without a key, a page that does not exist, a max_query that is too small, a NaN in a value that only later rows see"""
+    q, cache, table, n, start = lb.attention_case(dtype, dim, 16, 1, 16, [100, 93], [5, 7])
+    check = lambda *args, **kw: lb.check_attention(*args, p_terms=2, **kw)
+    with simlib.cus(1):
+        assert _path(q, cache, table, [5, 7]) == 3
+        check(simops.kv4_attention(q, cache, table, n, start, scale=-0.3), q, cache, table, n, start, scale=-0.3)
+        few = torch.tensor([2, 93], dtype=torch.int32)
+        out = simops.kv4_attention(q, cache, table, few, start)
+        check(out, q, cache, table, few, start)
+        assert (out[:3] == 0).all()
+        holes = table.clone()
+        holes[0, 1], holes[1, 0], holes[1, 4] = 10**6, -1, -1
+        check(simops.kv4_attention(q, cache, holes, n, start), q, cache, holes, n, start)
+        p, i = int(table[0, 98 // 16]), 98 % 16   # key 98: rows 3 and 4 of sequence 0 see it
+        vs = cache[3].clone()
+        vs[p, 0, i // 4, 1, i % 4] = 255
+        nan = (cache[0], cache[1], cache[2], vs)
+        out = simops.kv4_attention(q, nan, table, n, start)
+        check(out, q, nan, table, n, start)
+        assert torch.isnan(out[3:5, :, 32:64]).all() and not torch.isnan(out[:3]).any() and not torch.isnan(out[:, :, :32]).any()
+        ks = cache[1].clone()
+        ks[int(table[0, 1]), 0, 3, 1] = 255       # key 19: every row of sequence 0 sees it
+        nan = (cache[0], ks, *cache[2:])
+        out = simops.kv4_attention(q, nan, table, n, start)
+        check(out, q, nan, table, n, start)
+        assert torch.isnan(out[:5]).all() and not torch.isnan(out[5:]).any()
