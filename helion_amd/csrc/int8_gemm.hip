@@ -596,12 +596,13 @@ static void i8_offsets(I8Plan& p, int64_t M, int64_t N) {
   p.bytes = at;
 }
 
-// Up to 32 rows: k in pieces of at most 64 steps per workgroup (eight waves of up to eight), and in more of them while the
-// groups of 16 columns do not fill the compute units; at least eight steps each.
+// Up to 32 rows: k in pieces of at most 64 steps per workgroup (eight waves of up to eight), as few as that takes.  More of them,
+// for the compute units that the groups of 16 columns leave idle, cost more in partial sums and a second launch than they
+// give: 16 x 2048 x 2048 6.5 us, whole 3.6; 16 x 64 x 8192 8.8 and 5.9; 32 x 256 x 8192 9.9 and 8.2; 1 x 64 x 65536 in 64 pieces
+// 31.4, in eight 11.3; 16 x 1024 x 16384 in four 8.8, in two 9.2.
 static I8Plan i8_plan_skinny(I8Plan p, int64_t M, int64_t N, int64_t K) {
-  const int64_t nk = p.ka / I8_BK, ncg = (N + 15) / 16;
-  int64_t s = (nk + 63) / 64;
-  while (ncg * s < hx_cu_count() && nk / (2 * s) >= 8) s *= 2;
+  const int64_t nk = p.ka / I8_BK;
+  const int64_t s = (nk + 63) / 64;
   const int64_t per = ((nk + s - 1) / s + 7) / 8 * 8;
   p.bm = 16, p.bn = 16;
   p.splits = (int)((nk + per - 1) / per);

@@ -640,7 +640,7 @@ def test_kv4_attention_of_infinite_queries(dtype, group, kv_heads, pairs):
     (512, 4096, 4096, BF, BF, 2), (200, 515, 48, HF, BF, 18), (100, 512, 16000, BF, BF, 10), (130, 2048, 16400, None, HF, 26),
     (777, 4096, 4096, BF, BF, 3), (777, 4100, 4112, F32, HF, 19), (200, 4096, 16384, BF, BF, 11), (200, 4096, 16400, HF, HF, 27),
     (3500, 2560, 4096, BF, BF, 4), (3500, 2500, 4096, HF, F32, 4), (3500, 2560, 4112, F32, HF, 20),
-    (1, 256, 128, None, HF, 1), (16, 1024, 8192, BF, BF, 9), (16, 300, 1040, F32, F32, 17), (30, 64, 9008, HF, BF, 25),
+    (1, 256, 128, None, HF, 1), (16, 1024, 8192, BF, BF, 1), (16, 1000, 16384, BF, BF, 9), (16, 300, 1040, F32, F32, 17), (30, 64, 9008, HF, BF, 25),
 ])
 def test_int8_gemm_every_kernel(m, n, k, bias, out, path):
     """tiles of 64, 128 and 256 rows and the kernel for up to 32, unsplit and split, K a multiple of 128 and not, the output types"""

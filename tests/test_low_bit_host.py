@@ -193,6 +193,7 @@ def test_which_kernel_a_size_runs():
     gemm = lambda m, n, k, a=A, b=A: lib.hx_int8_gemm_path(m, n, k, k, 1, k, a, b)
     assert [gemm(*s) for s in ((16, 28672, 8192), (1, 64, 16384), (16, 300, 1040), (512, 4096, 4096), (128, 8192, 8192), (777, 4096, 4096),
                                (777, 4100, 4112), (200, 4096, 16384), (8192, 8192, 8192), (3500, 2560, 4112))] == [1, 9, 17, 2, 10, 3, 19, 11, 4, 20]
+    assert [gemm(*s) for s in ((16, 1024, 8192), (1, 1024, 4096), (16, 2048, 2048), (32, 256, 8192))] == [1] * 4  # splitting costs more than it gives
     assert gemm(8192, 8192, 8191) == 4 and gemm(777, 4100, 4112, A + 1) == 19 and gemm(777, 4100, 4112, A + 1, A + 1) == 3  # copies have whole k-tiles
     assert gemm(0, 4, 4) == 0 and gemm(4, 4, 200000) == 0
     att = lambda t, b, h, kv, d, page, width, mq, dt=1: lib.hx_kv4_attention_path(t, b, h, kv, d, page, width, mq, dt)

@@ -292,7 +292,7 @@ TILES = [
     (1, 257, 257, 1040, BF, BF, 20), (1, 300, 513, 784, HF, F32, 20), (1, 129, 256, 640, None, HF, 4), (1, 129, 256, 2048, BF, BF, 4),
     (4, 129, 256, 2064, F32, HF, 19), (4, 129, 256, 2048, BF, BF, 3), (3, 128, 128, 4096, BF, BF, 11), (8, 130, 128, 8208, None, HF, 27),
     (16, 250, 250, 4112, F32, BF, 26), (4, 100, 128, 4096, None, F32, 10), (2, 128, 128, 4096, HF, HF, 2), (2, 100, 128, 2064, None, BF, 18),
-    (1, 5, 40, 8192, BF, BF, 1), (4, 5, 40, 8192, None, HF, 9), (1, 20, 40, 8208, F32, F32, 25), (256, 20, 70, 1040, HF, BF, 17),
+    (1, 5, 40, 8192, BF, BF, 1), (4, 5, 40, 8320, None, HF, 9), (1, 20, 40, 8208, F32, F32, 25), (256, 20, 70, 1040, HF, BF, 17),
 ]
 
 
