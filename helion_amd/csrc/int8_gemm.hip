@@ -218,7 +218,8 @@ __global__ __launch_bounds__(256) void hx_int8_gemm_tile(I8Args p) {
 // blocks): under the first one the DMA of tile kt+2 goes out into this tile's own stage, whose fragments are all in
 // registers; between the halves "tile kt+1 has landed" is awaited; under the second the fragments of tile kt+1 replace
 // those that have had their last MFMA.  Rows past M or N re-read the last one and are not stored.
-// Bound by the matrix pipes and power: 8192 x 8192 x 8192 404 to 420 us, 2.6 to 2.7 POP/s, with an MFMA in 68 % of the busy
+// Bound by the matrix pipes and power: 8192 x 8192 x 8192 391 to 420 us, 2.6 to 2.8 POP/s, in runs of seconds; the first twenty
+// launches after idle take 407 to 519 while the clock finds its place.  An MFMA runs in 68 % of the busy
 // cycles (tiles of 128 x 128: 721 us, twice the LDS traffic per MFMA).
 // ------------------------------------------------------------------------------------------
 template <int OUT, bool KT>

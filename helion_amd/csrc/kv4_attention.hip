@@ -102,8 +102,8 @@ struct KaSeq {
 // The sequence that runs at place `at` of the batch's order: those with more keys first, so that what runs last is short.
 // Sequences i * n + g form group g of n groups of up to 64; the groups are taken in turn, each in the order of its lengths
 // (in 256 steps of the table's width, equal ones by their number): a lane per sequence, and the length's bits from the top
-// down tell in which half of those left the wanted place lies.  64 sequences of up to 2048 keys, 32 heads: 42.6 -> 36.7 us;
-// 24 of up to 4000 with 1 to 200 new tokens: 96 -> 86.
+// down tell in which half of those left the wanted place lies.  64 sequences of up to 2048 keys, 32 heads: 50.7 -> 40.9 us;
+// 24 of up to 4000 with 1 to 200 new tokens: 113 -> 103 (both in a graph).
 __device__ __forceinline__ int ka_longest_first(const KaArgs& a, int at) {
   const int n = (a.batch + 63) >> 6, g = n == 1 ? 0 : at % n, lane = threadIdx.x & 63;
   int k = n == 1 ? at : at / n;
@@ -132,8 +132,9 @@ __device__ __forceinline__ bool ka_sequence(const KaArgs& a, KaSeq& q) {  // fal
     if (a.last_first) q.block0 = a.blocks - 1 - q.block0;
     q.split = 0;
   } else {
-    // The blocks of one sequence run next to each other, as they read the same keys, and its last ones, which see the most,
-    // first: 24 sequences of up to 4000 keys with 1 to 200 new tokens 168 us block by block, 97 so, 94 with the last first.
+    // The blocks of one sequence run next to each other, as they read the same keys (24 sequences of up to 4000 keys with 1 to
+    // 200 new tokens, with one term a weight: 168 us block by block, 97 so), and its last ones, which see the most, first
+    // (2 x 512 tokens over 4096 keys 102.9 -> 100.3 us, head dim 64 71.0 -> 69.5; those 24 sequences 101 -> 103).
     q.block0 = a.blocks - 1 - id % a.blocks;
     id /= a.blocks;
     q.split = id % a.splits;
@@ -579,7 +580,9 @@ static KaPlan ka_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_h
   KaPlan p;
   // (a max_query that is padded, for a graph or by a server's limit, plans what the tokens need)
   const int64_t rows = (max_query < tokens ? max_query : tokens) * (heads / kv_heads);
-  // Two blocks of rows share a conversion of the keys and values; a head dim of 256 or an fp32 query leaves no registers for it.
+  // Two blocks of rows share a conversion of the keys and values.  A head dim of 256 leaves no registers for it (680 to 1640
+  // bytes of scratch a lane; 512 tokens over 4096 keys, bf16: 123 us with one block, 391 with two), nor does an fp32 query at
+  // 128 (196 bytes; 91 and 97); at 64, where it would give a tenth (61 and 55), fp32 goes the same way.
   p.rb = rows > 16 && D <= 128 && dt != HX_F32 ? 2 : 1;
   p.nw = 4;
   p.many = false;
@@ -603,7 +606,9 @@ static KaPlan ka_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_h
   // length, and what ends last counts) or two of the larger ones; a sequence shorter than the table's width uses fewer.
   // Where there are four per unit without a split the joining costs more than it gives (64 sequences x 32 heads of up to
   // 2048 keys: 42 us whole, 48 in two pieces).  One sequence of 32768 keys, 8 heads: pieces of 2048 18.4 us, 1024 14.0,
-  // 512 15.2; 32 sequences up to 32768: 122, 124, 125; 4 new tokens of 16 sequences of 8192: two per unit 40, four 47.
+  // 512 15.2; 32 sequences up to 32768: 122, 124, 125; 4 new tokens of 16 sequences of 8192: two per unit 46, four 51.
+  // Where there are four per unit, one much longer sequence is not split either: 128 sequences of 500 keys, 8 heads, one of
+  // 32768 among them take 169 us, most of it that one.
   const int64_t base = batch * kv_heads * blocks, cus = hx_cu_count(), most = max_keys / KA_PIECE;
   const int64_t want = base >= 4 * cus || p.many ? 1 : ((p.rb == 1 ? 16 : 2) * cus + base - 1) / base;
   int64_t s = want < most ? want : most;
@@ -704,7 +709,7 @@ extern "C" int hx_kv4_attention(const void* q, int64_t q_token_stride, int64_t q
   a.page_shift = __builtin_ctzll((unsigned long long)page), a.table_width = pages > 0 ? (int)table_width : 0, a.causal = causal != 0;
   a.splits = p.splits, a.blocks = p.blocks;
   // Workgroups of 128 rows in more than one round: the last blocks see the most keys and go first (4096 tokens over 4096
-  // keys 177 -> 163 us); in one round they start together, and the first ones first is better (338 and 323 us).
+  // keys 241 -> 210 us); in one round they start together, and the first ones first is better (2048 over 10240 460 and 440 us).
   const int64_t groups = batch * kv_heads * p.blocks * p.splits;
   a.longest_first = batch > 1 && groups > 2 * hx_cu_count();
   a.len_shift = 0;

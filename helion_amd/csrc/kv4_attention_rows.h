@@ -7,10 +7,10 @@
 // Every wave reads all fragments for its own two blocks of 16 rows; scores, statistics and outputs stay in its registers
 // and nothing is joined at the end.
 //
-// What bounds it (2048 new tokens of 32 heads over 10240 keys, head dim 128: bf16 438 us, 0.71 PFLOP/s of the formula's
+// What bounds it (2048 new tokens of 32 heads over 10240 keys, head dim 128: bf16 440 us, 0.70 PFLOP/s of the formula's
 // products; fp16 496): for 32 keys a wave's MFMAs take 832 cycles (16 for the scores, 32 for the two terms of the weights, 4 for
-// their sums, 16 cycles each), its vector instructions (a quarter of them exponentials at a quarter of the rate) about 650,
-// its 16 KB of fragments a quarter of 500 cycles of the LDS; two waves per SIMD hide little of that behind each other.
+// their sums, 16 cycles each), its vector instructions about 900, its 16 KB of fragments a quarter of 500 cycles of the LDS;
+// two waves per SIMD hide little of that behind each other (an MFMA runs in 49 % of the busy cycles, a vector instruction issues in 53).
 // Tried and slower (with one term a weight, 323 us): scores one half tile ahead in the wave (385), equal priorities (338).
 //
 // A sequence with at most 16 rows (a single token in a mixed batch) is worked on as in ka_few instead.
@@ -40,7 +40,7 @@ __global__ __launch_bounds__(KR_WAVES * 64, 2) void hx_kv4_attention_rows(KaArgs
   }
   KrLds<D>& lds = *(KrLds<D>*)raw;
   // Two waves share a SIMD, and with equal rights they drift into the same phase and wait for the same pipe: one of them
-  // goes first wherever both can (with one term a weight, 2048 new tokens over 10240 keys 338 -> 323 us, head dim 64 74 -> 66).
+  // goes first wherever both can (2048 new tokens over 10240 keys 461 -> 441 us, head dim 64 347 -> 328; 8 x 512 over 2048 176 -> 182).
   if (hx_wave_slot() & 1) __builtin_amdgcn_s_setprio(2);
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);

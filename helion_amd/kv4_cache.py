@@ -71,7 +71,8 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, block_table: torch.Tensor, s
 
     Rows of q outside ``query_start[0] .. query_start[sequences] - 1`` are left as they were in ``out``, which is allocated where it is
     not given (undefined there).  Table entries behind a sequence's last page are not used, and a page outside the cache masks
-    its keys.  Keys and values enter the products exactly, q and the weights as sums of bf16 terms, everything else is fp32."""
+    its keys; a length beyond the table counts as the table's size.  Keys and values enter the products exactly, q and the
+    weights as sums of bf16 terms (weights two, three for float32, in every batch), everything else is fp32."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     args = (q, *cache, block_table, seq_lens, query_start, max_query_len, float(scale), bool(causal))

@@ -334,7 +334,9 @@ int hx_kv4_read(const void* k_codes, const void* k_scales, const void* v_codes, 
  * alone when query_start is NULL (then tokens == batch).  Query head hq reads key/value head hq / (heads / kv_heads).
  *   out = softmax(scale * q k^T) v;  causal: new token i of n sees the keys up to seq_lens[b] - n + i, else all of them.
  * A row that sees no key gives zeros.  Rows of q outside every sequence are neither read nor written.  Table entries behind
- * the last page of a sequence are not used; the keys of a page that does not exist are masked, as are lengths beyond the table.
+ * the last page of a sequence are not used; the keys of a page that does not exist are masked; a
+ * length beyond the table counts as the table's size (the diagonal ends there).  An infinity or a NaN in q makes its row NaN.  The
+ * fp32 sums are divided at the end: |v| * 2^8 * keys has to stay below 2^128.
  * q [tokens][heads][D] of `dtype`, elements of a head contiguous, token and head strides in elements; out contiguous,
  * 16-byte aligned, same dtype.  max_query: the most new tokens of one sequence (sizes the launch, with `tokens` as its
  * limit, 1 where query_start is NULL; more are computed too, only slower).  Products of exact bf16 terms (1 for a bf16 q, 2 for fp16, 3 for fp32), fp32 sums and statistics.
