@@ -7,13 +7,14 @@
 // or an infinity in y gets that as its scale and zeros as its integers.
 //
 // Precision: the root cancels in y / max|y|, so the integers need only the products h * weight, which fp32 holds exactly for
-// 16-bit types (for fp32 they are rounded once), and a quotient rounded in fp64: a value next to the middle between two
-// integers falls to the formula's side.  (All in fp32 some thirty of a million integers fell to the other.)  The mean of
-// the squares is summed in fp64, where no square of an fp32 number overflows, and the scale is rounded once.
+// 16-bit types (for fp32 they are rounded once), and a quotient that is right next to a middle between two integers (see
+// SHORT): a value there falls to the formula's side.  (With plain fp32 quotients one to four of a million integers of a norm
+// fell to the other, and 117 of bf16 rows without one, whose quotients are often middles.)  The mean of the squares is summed
+// in fp64, where no square of an fp32 number overflows, and the scale is rounded once.
 //
 // Bound by memory: x (and the residual) are read once, h, q and the scale written once.  A row lives in the registers of
-// the lanes that share it, so neither the mean nor the maximum costs a second read; the two reductions go through the
-// wave's shuffles and, where several waves share a row, four or sixteen floats of LDS.  8192 x 8192 bf16 with a residual:
+// the lanes that share it, so neither the mean nor the maximum costs a second read; both are reduced together, through the
+// wave's shuffles and, where several waves share a row, a few numbers of LDS each.  8192 x 8192 bf16 with a residual:
 // 86 us, 470 MB at 5.5 TB/s; one row 4.6 us.
 #include "hx_common.h"
 

@@ -666,3 +666,18 @@ def test_kv4_attention_every_kernel(dtype, dim, page, kv_heads, group, lens, new
     assert _lib.load().hx_kv4_attention_path(q.shape[0], len(lens), q.shape[1], kv_heads, dim, page, table.shape[1], mq, 1 if dtype == BF else 0) == path
     out = hx.kv4_attention(q, cache, table, n, query_start=start, max_query_len=mq)
     lb.check_attention(out, q, cache, table, n, start)
+
+
+@pytest.mark.parametrize("dtype,residual,width,size,eps", [(BF, True, 130, 1.5e38, 1e-6), (BF, True, 8192, 1e-35, 1e-6), (F32, True, 33000, 1e-35, 0.0),
+                                                           (BF, False, 300, 1e-36, 0.0), (F32, False, 2100, 3e38, 0.0)])
+def test_rms_norm_int8_products_beyond_fp32(dtype, residual, width, size, eps):
+    """rows whose products with the weight leave fp32, or come near its lower end, are worked out again with a power of two"""
+    x, r, w = lb.norm_inputs(3, width, dtype, residual, 11)
+    x = (x.double() / x.double().abs().amax() * size).to(dtype)
+    r = (r.double() / r.double().abs().amax() * size).to(dtype) if residual else None
+    x[1, 0] = size                                   # (no row of zeros: without eps it has no root)
+    res = hx.rms_norm_int8(*_dev(x, w), residual=r.to(DEV) if residual else None, eps=eps)
+    h = ref.add(x, r)
+    lb.check_rows(res[0].cpu(), res[1].cpu(), ref.rms_norm(h, w, eps), 4)
+    if dtype == BF:
+        lb.check_border_rows(res[0].cpu(), h, w)

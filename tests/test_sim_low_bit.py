@@ -360,3 +360,18 @@ def test_kv4_attention_masks_with_128_rows_a_workgroup(dtype, dim):
         out = simops.kv4_attention(q, nan, table, n, start)
         check(out, q, nan, table, n, start)
         assert torch.isnan(out[:5]).all() and not torch.isnan(out[5:]).any()
+
+
+@pytest.mark.parametrize("dtype,residual,width,size,eps", [(BF, True, 130, 1.5e38, 1e-6), (BF, True, 700, 1e-35, 1e-6), (F32, True, 2100, 1e-35, 0.0),
+                                                           (BF, False, 300, 1e-36, 0.0), (F32, False, 515, 3e38, 0.0)])
+def test_rms_norm_int8_products_beyond_fp32(dtype, residual, width, size, eps):
+    """rows whose products with the weight leave fp32, or come near its lower end, are worked out again with a power of two"""
+    x, r, w = lb.norm_inputs(3, width, dtype, residual, 11)
+    x = (x.double() / x.double().abs().amax() * size).to(dtype)
+    r = (r.double() / r.double().abs().amax() * size).to(dtype) if residual else None
+    x[1, 0] = size                                   # (no row of zeros: without eps it has no root)
+    q, scale, h = simops.rms_norm_int8(x, w, r, eps)
+    h = ref.add(x, r)
+    lb.check_rows(q, scale, ref.rms_norm(h, w, eps), 4)
+    if dtype == BF:
+        lb.check_border_rows(q, h, w)
