@@ -156,16 +156,25 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void hx_norm_int8_kernel(
     for (int v = 0; v < V; ++v)
 #pragma unroll
       for (int e = 0; e < NQ_EPV; ++e) ss = fma((double)y[v][e], (double)y[v][e], ss);
-    times_weight(1.f, t);
+    if (DT != HX_F32) times_weight(1.f, t);
   }
-  unsigned top = largest();
+  unsigned top = NORM && DT == HX_F32 ? 0 : largest();
   nq_join<TPR, NORM>(ss, top, lds, 0);
   float unit = 1.f;  // the formula's y is what is in the registers / (unit * rms)
-  if (NORM && DT != HX_F16 && (top >= 0x7F800000u || (top < 0x0D800000u && ss > 0.))) {
-    // The largest product has left fp32 or come near its lower end (2^-100): once more, with a power of two near 1 / rms.
+  auto near_one = [&]() {  // a power of two near 1 / rms
     const uint64_t mean = __builtin_bit_cast(uint64_t, fma(ss, by_width, (double)eps));
     const int e2 = 1023 - (int)((mean >> 52) & 0x7FF);
-    unit = __uint_as_float((uint32_t)(min(max(e2 >> 1, -126), 127) + 127) << 23);
+    return __uint_as_float((uint32_t)(min(max(e2 >> 1, -126), 127) + 127) << 23);
+  };
+  if (NORM && DT == HX_F32) {
+    // (one after the other: the second pass below would spill where rows are long, 1024 x 65536 370 us against 316)
+    unit = near_one();
+    times_weight(unit, t);
+    top = largest();
+    nq_join<TPR, false>(ss, top, lds, 1);
+  } else if (NORM && DT == HX_BF16 && (top >= 0x7F800000u || (top < 0x0D800000u && ss > 0.))) {
+    // The largest product has left fp32 or come near its lower end (2^-100): once more, with that power.
+    unit = near_one();
     int lane = t;
     HX_OPAQUE_V(lane);  // (addresses of its own: those of the first loads would take their registers all along)
 #pragma unroll
